@@ -293,6 +293,77 @@ int xp_encode_rows(const void *raw, int64_t rows, int64_t n, int64_t pitch, int6
                    void *records, void *luts, int64_t *used, void *scratch,
                    int64_t scratch_bytes, void *stream);
 
+/* ---- routing: what comes before a step's topk_ids ----
+ *
+ * No counterpart in the reference, which takes topk_ids from vLLM's router.
+ * logits[T] rows of E values (dtype XP_F32, XP_BF16 or XP_F16), `stride`
+ * elements from one row to the next.  valid (may be NULL): uint8[T], 0 for a row
+ * that holds no token (padding); nothing of such a row is read. */
+
+/* Element types of logits and activations. */
+#define XP_F32 0
+#define XP_BF16 1
+#define XP_F16 2
+/* Limits of the routing and low-rank entry points: experts a token is routed
+ * to, and rows of a call (larger values are XP_ERANGE, as is T * topk above
+ * 2^31 - 1). */
+#define XP_MAX_TOPK 32
+#define XP_MAX_TOKENS (1 << 26)
+
+/* The topk experts of every token with the largest logits, in descending order
+ * (equal logits: the lower expert first; NaN counts as the largest value; -inf
+ * is never chosen: the remaining ids are -1 and their weights 0), ids[T][topk].
+ * weights[T][topk]: the softmax probabilities of the chosen experts, divided by
+ * their sum when renormalize is not 0.  counts[E]: the choices of each expert.
+ * tokens[1] (may be NULL): the number of rows that are valid.  loss (may be NULL) receives the balance loss E * sum_e f_e P_e with f_e = counts[e] /
+ * (tokens * topk) and P_e the mean probability of e over the tokens; 0 without
+ * tokens.  scratch: xp_route_scratch_bytes(T, E) bytes of device memory, 4-byte
+ * aligned (NULL when that is 0), not shared by calls that may overlap. */
+int64_t xp_route_scratch_bytes(int64_t T, int64_t E);
+int xp_route(const void *logits, int dtype, int64_t T, int64_t E, int64_t stride,
+             const uint8_t *valid, int64_t topk, int renormalize, float *weights, int32_t *ids,
+             int64_t *counts, int64_t *tokens, float *loss, void *scratch, int64_t scratch_bytes,
+             void *stream);
+
+/* counts[E], tokens[1] and the balance loss as xp_route gives them, for a routing
+ * chosen elsewhere: ids[T][topk] (contiguous; ids outside [0, E) are not
+ * counted, equal ids of a row are counted each). */
+int xp_balance(const void *logits, int dtype, int64_t T, int64_t E, int64_t stride,
+               const uint8_t *valid, const void *ids, int ids_bytes, int64_t topk,
+               int64_t *counts, int64_t *tokens, float *loss, void *scratch,
+               int64_t scratch_bytes, void *stream);
+
+/* grad[T][E] (contiguous, dtype as logits): the gradient of the logits.
+ * grad_weights[T][topk] (NULL: none) is the gradient of xp_route's weights for
+ * the ids that it wrote; grad_loss (NULL: none) points at the gradient of the
+ * loss, with counts and tokens as the forward call wrote them.  Rows that are not valid
+ * get zeros. */
+int xp_route_backward(const void *logits, int dtype, int64_t T, int64_t E, int64_t stride,
+                      const uint8_t *valid, const int32_t *ids, int64_t topk, int renormalize,
+                      const float *grad_weights, const int64_t *counts, const int64_t *tokens,
+                      const float *grad_loss, void *grad, void *stream);
+
+/* ---- low-rank adapters of many requests ----
+ *
+ * No counterpart in the reference.  out[m] = y[m] + scale[s] * (x[m] A_s^T) B_s^T
+ * for every row m < M, where s is the slot of the row's adapter: ids[m], or
+ * slot_of[ids[m]] when slot_of (int32[adapters], an expert_map of
+ * xp_acquire_pair) is not NULL.  A row whose id or slot is out of range has no
+ * adapter: out[m] = y[m].  x: M rows of H values, y and out: M rows of N values,
+ * a: [slots][r][H], b: [slots][N][r] (both contiguous), all of type dtype
+ * (XP_BF16 or XP_F16); the strides count elements from row to row.  scale:
+ * float[slots], NULL for ones.  out may be y itself (with the same stride) and
+ * overlaps no other operand.  r <= XP_MAX_RANK.  scratch:
+ * xp_low_rank_scratch_bytes(M, slots) bytes of device memory, 16-byte aligned
+ * (NULL when that is 0), not shared by calls that may overlap. */
+#define XP_MAX_RANK 128
+int64_t xp_low_rank_scratch_bytes(int64_t M, int64_t slots);
+int xp_add_low_rank(const void *x, int64_t x_stride, const void *y, int64_t y_stride, void *out,
+                    int64_t out_stride, int dtype, int64_t M, int64_t H, int64_t N, int64_t r,
+                    const void *a, const void *b, int64_t slots, const float *scale,
+                    const void *ids, int ids_bytes, const int32_t *slot_of, int64_t adapters,
+                    void *scratch, int64_t scratch_bytes, void *stream);
+
 /* ---- host side ---- */
 
 /* Replaces codec.encode (codec.py:125-193) on the host: compress raw[n] into

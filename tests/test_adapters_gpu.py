@@ -1,0 +1,294 @@
+"""Low-rank adapters against a 64-bit restatement.
+
+Bound of an output: half a step of its type, and the fp32 work before it.  A sum of
+H products in 32 bits is off by at most H steps of 2^-23 of the sum of magnitudes
+(tensor cores may cut instead of rounding); the low-rank value may be carried as two
+16-bit parts, which keeps 2^-16 of it; the second product adds rank steps, the scale
+and the final addition two more.
+"""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda")
+STEP = 2.0 ** -23
+HALF = {torch.bfloat16: (2.0 ** -8, 2.0 ** -134), torch.float16: (2.0 ** -11, 2.0 ** -25)}
+TYPES = [torch.bfloat16, torch.float16]
+
+
+def make(M, H, N, r, S, dtype, seed=0, size=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+
+    def n(*shape):
+        return torch.randn(shape, generator=g, device=DEV)
+
+    o = dict(x=n(M, H) * size, y=n(M, N), a=n(S, r, H) / math.sqrt(H), b=n(S, N, r) / math.sqrt(r))
+    o = {k: v.to(dtype) for k, v in o.items()}
+    o["scale"] = torch.rand((S,), generator=g, device=DEV) + 0.5
+    return o, g
+
+
+def reference(y, x, a, b, slots, scale):
+    """The rows' results and their bounds, for slots (-1: no adapter) on the host."""
+    M, N = y.shape
+    S, r, H = a.shape
+    want, bound = y.double().clone(), torch.zeros((M, N), dtype=torch.float64, device=DEV)
+    half, tiny = HALF[y.dtype]
+    for s in sorted(set(slots.tolist()) - {-1}):
+        m = (slots == s).nonzero().reshape(-1)
+        f = 1.0 if scale is None else scale[s].double()
+        xs, A, B = x[m].double(), a[s].double(), b[s].double()
+        v, size = xs @ A.T, xs.abs() @ A.abs().T
+        low = f * (v @ B.T)
+        off = f * (((H + 2) * STEP * size + 2.0 ** -16 * v.abs()) @ B.abs().T
+                   + (r + 4) * STEP * (v.abs() @ B.abs().T))
+        want[m] += low
+        bound[m] = half * 1.01 * want[m].abs() + tiny + off * 1.01 + 2 * STEP * (y[m].double().abs()
+                                                                                + low.abs())
+    return want, bound
+
+
+def check(o, ids, slots, scale="own", out=None, **more):
+    from vllm_expert_pager import adapters
+
+    scale = o["scale"] if isinstance(scale, str) else scale
+    y, x = o["y"], o["x"]
+    want, bound = reference(y, x, o["a"], o["b"], slots, scale)
+    got = adapters.add_low_rank(y, x, o["a"], o["b"], ids, scale=scale, out=out, **more)
+    torch.cuda.synchronize()
+    bad = (got.double() - want).abs() > bound
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} values off, first at " \
+        f"{bad.nonzero()[0].tolist()}, rows {sorted(set(bad.nonzero()[:, 0].tolist()))[:9]}"
+    return got
+
+
+def fresh(o):
+    return torch.full_like(o["y"], math.nan)
+
+
+def patterns(M, S, g):
+    """Row -> slot of the batches that a server sees."""
+    i = torch.arange(M, device=DEV)
+    yield "one adapter", torch.full((M,), S - 1, device=DEV)
+    yield "each its own", i % S
+    yield "prompts", (i * 5 // max(M, 1)) % S
+    yield "any order", torch.randint(-1, S, (M,), generator=g, device=DEV)
+    yield "none", torch.full((M,), -1, device=DEV)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("H, N, r", [(2048, 1024, 16), (64, 64, 8), (512, 2048, 64), (96, 40, 128),
+                                     (1000, 72, 24), (8, 8, 1)])
+@pytest.mark.parametrize("M", [1, 2, 7, 8, 9, 33, 64, 65, 130])
+def test_add_low_rank_matches_the_definition(dtype, H, N, r, M):
+    S = 6
+    o, g = make(M, H, N, r, S, dtype, seed=M + r)
+    for _, slots in patterns(M, S, g):
+        check(o, slots.to(torch.int32), slots, out=fresh(o))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("H, N, r", [(1, 1, 1), (3, 5, 2), (1021, 2047, 13), (65, 129, 3),
+                                     (63, 1000, 17), (2047, 31, 127), (8, 24, 65), (24, 7, 16),
+                                     (130, 66, 33)])
+@pytest.mark.parametrize("M", [1, 5, 64, 300])
+def test_sizes_that_no_vector_divides(dtype, H, N, r, M):
+    S = 5
+    o, g = make(M, H, N, r, S, dtype, seed=M + r)
+    for _, slots in patterns(M, S, g):
+        check(o, slots.to(torch.int64), slots, out=fresh(o))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M, H, N, r, S", [
+    (255, 256, 512, 16, 200), (256, 128, 256, 64, 3), (257, 256, 128, 8, 64),
+    (1023, 64, 192, 32, 7), (1024, 128, 128, 16, 1), (1025, 128, 128, 16, 300),
+    (2048, 512, 2048, 16, 8), (4099, 250, 130, 13, 11), (5000, 512, 256, 64, 4096),
+    (9001, 64, 64, 128, 2)])
+def test_long_batches(dtype, M, H, N, r, S):
+    o, g = make(M, H, N, r, S, dtype, seed=M)
+    for name, slots in patterns(M, S, g):
+        if name == "each its own" and S > 300:
+            slots = slots % 50 * 7
+        elif name == "any order" and S > 300:
+            slots = torch.where(slots >= 0, slots % 40 * 100, -1)
+        check(o, slots.to(torch.int32), slots, out=fresh(o))
+    # A long prompt between single tokens.
+    slots = torch.arange(M, device=DEV) % min(S, 40)
+    slots[20 : M - 30] = S - 1
+    check(o, slots.to(torch.int32), slots, out=fresh(o))
+
+
+@pytest.mark.parametrize("M", [4, 300, 3000])
+def test_in_place_and_ids_out_of_range(M):
+    S = 4
+    o, g = make(M, 128, 96, 16, S, torch.bfloat16, seed=M)
+    slots = torch.randint(-1, S, (M,), generator=g, device=DEV)
+    odd = torch.tensor([-1, -7, S, 1 << 40, -(1 << 62), (1 << 32) + 1], device=DEV)
+    ids = torch.where(slots >= 0, slots, odd[torch.arange(M, device=DEV) % 6])
+    before = o["y"].clone()
+    want, bound = reference(before, o["x"], o["a"], o["b"], slots, o["scale"])
+    from vllm_expert_pager import adapters
+
+    got = adapters.add_low_rank(o["y"], o["x"], o["a"], o["b"], ids, scale=o["scale"])
+    assert got is o["y"]
+    assert ((got.double() - want).abs() <= bound).all()
+    assert torch.equal(got[slots < 0], before[slots < 0])
+
+
+@pytest.mark.parametrize("M", [9, 200, 2500])
+def test_slot_map(M):
+    """Adapter ids through an expert_map: entries of -1, slots and ids out of range."""
+    S, num = 5, 64
+    o, g = make(M, 256, 64, 8, S, torch.float16, seed=M)
+    slot_map = torch.full((num,), -1, dtype=torch.int32, device=DEV)
+    slot_map[torch.arange(S, device=DEV) * 11] = torch.arange(S, dtype=torch.int32, device=DEV)
+    slot_map[63] = S        # a slot that the slab does not have
+    slot_map[62] = 1 << 30
+    ids = torch.randint(-2, num + 3, (M,), generator=g, device=DEV)
+    slots = torch.where((ids >= 0) & (ids < num), slot_map[ids.clamp(0, num - 1)].long(), -1)
+    slots[slots >= S] = -1
+    for t in (torch.int32, torch.int64):
+        check(o, ids.to(t), slots, slot_map=slot_map, out=fresh(o))
+    check(o, slots.to(torch.int32), slots, scale=None, out=fresh(o))
+
+
+@pytest.mark.parametrize("M", [3, 70, 1500])
+def test_what_no_row_uses_is_not_read(M):
+    """NaN and inf in free slots, in rows without an adapter's x, and around strided rows."""
+    S = 6
+    H, N, r = 192, 136, 24
+    o, g = make(M, H, N, r, S, torch.bfloat16, seed=M)
+    o["a"][4:], o["b"][4:], o["scale"][4:] = math.nan, math.inf, math.nan
+    slots = torch.randint(-1, 4, (M,), generator=g, device=DEV)
+    o["x"][slots < 0] = math.nan
+    for offset in (0, 8, 3):  # rows at any distance and alignment
+        wide = {k: torch.full((M, 400), math.nan, dtype=torch.bfloat16, device=DEV)
+                for k in ("x", "y", "out")}
+        x = wide["x"][:, offset : offset + H]
+        y = wide["y"][:, offset : offset + N]
+        out = wide["out"][:, offset : offset + N]
+        x.copy_(o["x"])
+        y.copy_(o["y"])
+        check({**o, "x": x, "y": y}, slots.to(torch.int32), slots, out=out)
+        rest = torch.ones((400,), dtype=torch.bool, device=DEV)
+        rest[offset : offset + N] = False
+        assert wide["out"][:, rest].isnan().all()  # the columns around out stay as they were
+    # y and x may be columns of one buffer, and out y itself.
+    both = torch.zeros((M, H + N), dtype=torch.bfloat16, device=DEV)
+    both[:, :H], both[:, H:] = o["x"], o["y"]
+    ref, bound = reference(o["y"], o["x"], o["a"], o["b"], slots, o["scale"])
+    from vllm_expert_pager import adapters
+
+    got = adapters.add_low_rank(both[:, H:], both[:, :H], o["a"], o["b"], slots,
+                                scale=o["scale"])
+    assert ((got.double() - ref).abs() <= bound).all()
+    keep = both[:, :H]
+    assert torch.equal(keep.isnan(), o["x"].isnan())
+
+
+@pytest.mark.parametrize("M", [2, 40, 1200])
+def test_rows_are_apart(M):
+    """A row's result is the same bits whatever rows it shares the batch with, in any order."""
+    S = 7
+    from vllm_expert_pager import adapters
+
+    o, g = make(M, 320, 200, 16, S, torch.bfloat16, seed=M)
+    slots = torch.randint(-1, S, (M,), generator=g, device=DEV).to(torch.int32)
+    first = adapters.add_low_rank(o["y"], o["x"], o["a"], o["b"], slots, out=fresh(o))
+    for _ in range(2):
+        again = adapters.add_low_rank(o["y"], o["x"], o["a"], o["b"], slots, out=fresh(o))
+        assert torch.equal(first, again)
+    perm = torch.randperm(M, generator=g, device=DEV)
+    moved = adapters.add_low_rank(o["y"][perm], o["x"][perm], o["a"], o["b"], slots[perm])
+    assert torch.equal(moved, first[perm])
+
+
+def test_large_and_small_values():
+    """Low-rank values beyond float16's range and deep below it keep their precision; an
+    infinity or NaN stays in its row."""
+    for M in (6, 400):
+        for size in (1e4, 1e-4):
+            o, g = make(M, 64, 32, 8, 3, torch.float16, seed=M, size=size)
+            slots = torch.arange(M, device=DEV) % 3
+            if size > 1:  # v around 3e5, scaled back into range
+                o["a"] = (o["a"].float() * 30).to(torch.float16)
+                o["scale"] = torch.full((3,), 2.0 ** -12, device=DEV)
+            check(o, slots, slots, out=fresh(o))
+        o, g = make(M, 64, 32, 8, 3, torch.float16, seed=M)
+        slots = torch.arange(M, device=DEV) % 3
+        clean = check(o, slots, slots, out=fresh(o))
+        o["x"][2, 5] = math.nan
+        o["x"][3, 7] = math.inf
+        from vllm_expert_pager import adapters
+
+        got = adapters.add_low_rank(o["y"], o["x"], o["a"], o["b"], slots, scale=o["scale"],
+                                    out=fresh(o))
+        assert got[2].isnan().all() and not got[3].isfinite().any()
+        rest = [i for i in range(M) if i not in (2, 3)]
+        assert torch.equal(got[rest], clean[rest])
+
+
+@pytest.mark.parametrize("big", ["x", "y"])
+def test_offsets_past_32_bits(big):
+    H, N, r, S, pitch = 128, 96, 16, 2, (1 << 30) + 8
+    for M, step in ((3, pitch), (1100, (1 << 21) + 8)):
+        o, _ = make(M, H, N, r, S, torch.bfloat16, seed=M)
+        slots = torch.arange(M, device=DEV) % S
+        width = H if big == "x" else N
+        buf = torch.empty(((M - 1) * step + width,), dtype=torch.bfloat16, device=DEV)
+        rows = buf.as_strided((M, width), (step, 1))
+        rows.copy_(o[big])
+        o[big] = rows
+        if big == "x":
+            check(o, slots, slots, out=fresh(o))
+        else:
+            want, bound = reference(o["y"].clone(), o["x"], o["a"], o["b"], slots, o["scale"])
+            from vllm_expert_pager import adapters
+
+            got = adapters.add_low_rank(rows, o["x"], o["a"], o["b"], slots, scale=o["scale"])
+            assert ((got.double() - want).abs() <= bound).all()
+        del buf, rows, o
+
+
+@pytest.mark.parametrize("M", [5, 1300])
+def test_replays_in_graphs_and_on_streams(M):
+    from vllm_expert_pager import adapters
+
+    S = 4
+    o, g = make(M, 256, 128, 16, S, torch.bfloat16, seed=M)
+    ids = torch.zeros((M,), dtype=torch.int32, device=DEV)
+
+    def step(out=None):
+        return adapters.add_low_rank(o["y"], o["x"], o["a"], o["b"], ids, scale=o["scale"],
+                                     out=torch.empty_like(o["y"]) if out is None else out)
+
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graphs.append((graph, out))
+    for seed in range(3):
+        ids.copy_(torch.randint(-1, S, (M,), generator=g, device=DEV))
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        slots = ids.long()
+        check(o, ids, slots, out=fresh(o))
+        assert all(torch.equal(out, want) for _, out in graphs)
+    sides = [torch.cuda.Stream() for _ in range(3)]
+    outs = []
+    for s in sides:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs.append(step())
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for out in outs)

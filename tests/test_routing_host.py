@@ -1,0 +1,168 @@
+"""Refusals of the routing entry points: none of them reaches a GPU.
+
+The C ABI checks its arguments before any CUDA call, the Python functions before
+the C ABI (fake tensors stand for CUDA ones where a later check is the subject).
+"""
+
+import ctypes
+
+import pytest
+import torch
+
+from vllm_expert_pager import native, routing
+
+BUF = (ctypes.c_uint8 * 4096)()
+P = ctypes.addressof(BUF)
+
+
+def xp_route(logits=P, dtype=0, T=4, E=8, stride=8, valid=None, topk=2, renorm=1, weights=P,
+             ids=P, counts=P, tokens=None, loss=None, scratch=None, scratch_bytes=0):
+    return native.lib().xp_route(logits, dtype, T, E, stride, valid, topk, renorm, weights, ids,
+                                 counts, tokens, loss, scratch, scratch_bytes, None)
+
+
+def xp_balance(logits=P, dtype=0, T=4, E=8, stride=8, valid=None, ids=P, ids_bytes=4, topk=2,
+               counts=P, tokens=None, loss=P, scratch=None, scratch_bytes=0):
+    return native.lib().xp_balance(logits, dtype, T, E, stride, valid, ids, ids_bytes, topk,
+                                   counts, tokens, loss, scratch, scratch_bytes, None)
+
+
+def xp_backward(logits=P, dtype=0, T=4, E=8, stride=8, valid=None, ids=P, topk=2, renorm=1,
+                grad_weights=P, counts=P, tokens=P, grad_loss=P, grad=P):
+    return native.lib().xp_route_backward(logits, dtype, T, E, stride, valid, ids, topk, renorm,
+                                          grad_weights, counts, tokens, grad_loss, grad, None)
+
+
+@pytest.mark.parametrize("change, status", [
+    ({"dtype": 3}, native.XP_EINVAL), ({"dtype": -1}, native.XP_EINVAL),
+    ({"T": -1}, native.XP_EINVAL), ({"E": 0}, native.XP_EINVAL),
+    ({"E": 4097}, native.XP_ERANGE), ({"T": (1 << 26) + 1}, native.XP_ERANGE),
+    ({"stride": -8}, native.XP_EINVAL), ({"topk": 0}, native.XP_EINVAL),
+    ({"topk": 9}, native.XP_EINVAL), ({"E": 64, "stride": 64, "topk": 33}, native.XP_ERANGE),
+    ({"logits": None}, native.XP_EINVAL), ({"weights": None}, native.XP_EINVAL),
+    ({"ids": None}, native.XP_EINVAL), ({"counts": None}, native.XP_EINVAL),
+    # Several CTAs: the sum over them needs scratch.
+    ({"T": 4096}, native.XP_EINVAL),
+    ({"T": 4096, "scratch": P, "scratch_bytes": 64}, native.XP_EINVAL),
+    ({"T": 4096, "scratch": P + 1, "scratch_bytes": 1 << 30}, native.XP_EINVAL),
+])
+def test_route_checks_its_arguments(change, status):
+    assert xp_route(**change) == status
+
+
+@pytest.mark.parametrize("change, status", [
+    ({"ids_bytes": 2}, native.XP_EINVAL), ({"ids": None}, native.XP_EINVAL),
+    ({"loss": None}, native.XP_EINVAL), ({"counts": None}, native.XP_EINVAL),
+    ({"dtype": 7}, native.XP_EINVAL), ({"E": 5000}, native.XP_ERANGE),
+    # A count of all choices would not fit 32 bits.
+    ({"T": 1 << 20, "topk": 1 << 11}, native.XP_ERANGE), ({"T": 4096}, native.XP_EINVAL),
+])
+def test_balance_checks_its_arguments(change, status):
+    assert xp_balance(**change) == status
+
+
+@pytest.mark.parametrize("change, status", [
+    ({"topk": 40}, native.XP_ERANGE), ({"ids": None}, native.XP_EINVAL),
+    ({"grad": None}, native.XP_EINVAL), ({"counts": None}, native.XP_EINVAL),
+    ({"tokens": None}, native.XP_EINVAL), ({"logits": None}, native.XP_EINVAL),
+    ({"E": 0}, native.XP_EINVAL), ({"T": 0}, native.XP_OK),
+])
+def test_backward_checks_its_arguments(change, status):
+    assert xp_backward(**change) == status
+
+
+def test_scratch_size():
+    need = native.lib().xp_route_scratch_bytes
+    assert need(0, 256) == 0 and need(1, 256) == 0
+    assert need(1 << 16, 256) % 4 == 0 and need(1 << 16, 256) > 0
+    assert need(1 << 26, 256) == need(1 << 16, 256)  # the launch's CTAs are bounded
+    assert need(-1, 256) == -1 and need(1, 0) == -1 and need(1, 5000) == -1
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros((4, 8))
+    with pytest.raises(ValueError, match="expected a CUDA tensor"):
+        routing.route(x, 2)
+    with pytest.raises(ValueError, match="expected a CUDA tensor"):
+        routing.balance_loss(x, torch.zeros((4, 2), dtype=torch.int32))
+
+
+@pytest.fixture
+def any_device(monkeypatch):
+    """Lets CPU tensors pass for CUDA ones: the checks behind the first are the subject."""
+    monkeypatch.setattr(native, "require_cuda", lambda *t: None)
+
+    def never(*a, **k):
+        raise AssertionError("a refused call reached the library")
+
+    monkeypatch.setattr(native, "launch", never)
+
+
+def test_route_refusals(any_device):
+    x = torch.zeros((4, 8))
+    for bad in (torch.zeros((4, 8), dtype=torch.float64), torch.zeros((4, 8), dtype=torch.int32),
+                torch.zeros((8,)), torch.zeros((2, 4, 8))):
+        with pytest.raises(ValueError, match="logits must be"):
+            routing.route(bad, 2)
+    with pytest.raises(ValueError, match="experts are supported"):
+        routing.route(torch.zeros((2, 4097)), 2)
+    with pytest.raises(ValueError, match="experts are supported"):
+        routing.route(torch.zeros((2, 0)), 1)
+    for k in (0, -1, 9):
+        with pytest.raises(ValueError, match="topk must be between 1 and 8"):
+            routing.route(x, k)
+    with pytest.raises(ValueError, match="topk must be between 1 and 32"):
+        routing.route(torch.zeros((2, 64)), 33)
+    for bad in (torch.ones((5,), dtype=torch.bool), torch.ones((4, 1), dtype=torch.bool),
+                torch.ones((4,))):
+        with pytest.raises(ValueError, match="valid must be"):
+            routing.route(x, 2, valid=bad)
+
+
+def test_balance_refusals(any_device):
+    x = torch.zeros((4, 8))
+    for bad in (torch.zeros((4,), dtype=torch.int32), torch.zeros((3, 2), dtype=torch.int32),
+                torch.zeros((4, 0), dtype=torch.int32)):
+        with pytest.raises(ValueError, match="topk_ids must be"):
+            routing.balance_loss(x, bad)
+    for bad in (torch.zeros((4, 2)), torch.zeros((4, 2), dtype=torch.bool)):
+        with pytest.raises(ValueError, match="must be integers"):
+            routing.balance_loss(x, bad)
+    with pytest.raises(ValueError, match="valid must be"):
+        routing.balance_loss(x, torch.zeros((4, 2), dtype=torch.int32),
+                             valid=torch.ones((3,), dtype=torch.bool))
+
+
+def test_launch_enters_the_tensors_device(monkeypatch):
+    """A call on tensors of another device than the current one is made with theirs current,
+    on their current stream; a status becomes an error."""
+    seen, current = [], [0]
+
+    class Device:
+        def __init__(self, d):
+            self.index = d.index
+
+        def __enter__(self):
+            self.was, current[0] = current[0], self.index
+
+        def __exit__(self, *a):
+            current[0] = self.was
+
+    class Stream:
+        def __init__(self, d):
+            self.cuda_stream = 1000 + d.index
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "current_stream", Stream)
+
+    def fn(x, stream):
+        seen.append((x, stream, current[0]))
+        return 0
+
+    native.launch(torch.device("cuda", 0), "f", fn, 1)
+    native.launch(torch.device("cuda", 3), "f", fn, 2)
+    assert seen == [(1, 1000, 0), (2, 1003, 3)] and current[0] == 0
+    with pytest.raises(ValueError, match="f failed"):
+        native.launch(torch.device("cuda", 3), "f", lambda stream: native.XP_EINVAL)
+    assert current[0] == 0

@@ -68,6 +68,16 @@ _SIGNATURES = {
     "xp_encode_row": (_i32, [_p, _i64, _i64, _i64, _p, _p, ctypes.POINTER(_i64)]),
     "xp_encode_scratch_bytes": (_i64, [_i64, _i64, _i64]),
     "xp_encode_rows": (_i32, [_p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p]),
+    "xp_route_scratch_bytes": (_i64, [_i64, _i64]),
+    "xp_route": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i64, _i32, _p, _p, _p, _p, _p, _p, _i64,
+                        _p]),
+    "xp_balance": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _p, _i32, _i64, _p, _p, _p, _p, _i64,
+                          _p]),
+    "xp_route_backward": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _p, _i64, _i32, _p, _p, _p, _p,
+                                 _p, _p]),
+    "xp_low_rank_scratch_bytes": (_i64, [_i64, _i64]),
+    "xp_add_low_rank": (_i32, [_p, _i64, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _i64, _p, _p,
+                               _i64, _p, _p, _i32, _p, _i64, _p, _i64, _p]),
     "xp_pinned_alloc": (_i32, [_i64, _i32, ctypes.POINTER(_p), ctypes.POINTER(_p)]),
     "xp_pinned_free": (_i32, [_p, _i64]),
     "xp_device_pointer": (_i32, [_p, ctypes.POINTER(_p)]),
@@ -87,6 +97,13 @@ XP_OK = 0
 XP_EINVAL = -22
 XP_ERANGE = -34
 XP_EPITCH = -75
+
+# Element types and limits of the routing and low-rank entry points.
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_EXPERTS = 4096
+MAX_TOPK = 32
+MAX_RANK = 128
+MAX_TOKENS = 1 << 26
 
 _lib: ctypes.CDLL | None = None
 
@@ -125,6 +142,17 @@ def ptr(t: torch.Tensor | None) -> int | None:
 def stream_of(device: torch.device) -> int:
     """Handle of the current CUDA stream of ``device`` (captured streams included)."""
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def launch(device: torch.device, what: str, fn, *args) -> None:
+    """Call ``fn(*args, stream)`` on the current stream of ``device``, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc != XP_OK:
+        check(rc, what)
 
 
 def require_cuda(*tensors: torch.Tensor | None) -> None:
