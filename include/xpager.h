@@ -336,7 +336,8 @@ int xp_balance(const void *logits, int dtype, int64_t T, int64_t E, int64_t stri
 /* grad[T][E] (contiguous, dtype as logits): the gradient of the logits.
  * grad_weights[T][topk] (NULL: none) is the gradient of xp_route's weights for
  * the ids that it wrote; grad_loss (NULL: none) points at the gradient of the
- * loss, with counts and tokens as the forward call wrote them.  Rows that are not valid
+ * loss, with counts and tokens as the forward call wrote them (tokens may be
+ * NULL when valid is: all rows are tokens).  Rows that are not valid
  * get zeros. */
 int xp_route_backward(const void *logits, int dtype, int64_t T, int64_t E, int64_t stride,
                       const uint8_t *valid, const int32_t *ids, int64_t topk, int renormalize,
@@ -353,10 +354,12 @@ int xp_route_backward(const void *logits, int dtype, int64_t T, int64_t E, int64
  * a: [slots][r][H], b: [slots][N][r] (both contiguous), all of type dtype
  * (XP_BF16 or XP_F16); the strides count elements from row to row.  scale:
  * float[slots], NULL for ones.  out may be y itself (with the same stride) and
- * overlaps no other operand.  r <= XP_MAX_RANK.  scratch:
+ * overlaps no other operand.  r <= XP_MAX_RANK, slots <= XP_MAX_ADAPTER_SLOTS
+ * (else XP_ERANGE).  scratch:
  * xp_low_rank_scratch_bytes(M, slots) bytes of device memory, 16-byte aligned
  * (NULL when that is 0), not shared by calls that may overlap. */
 #define XP_MAX_RANK 128
+#define XP_MAX_ADAPTER_SLOTS 8192
 int64_t xp_low_rank_scratch_bytes(int64_t M, int64_t slots);
 int xp_add_low_rank(const void *x, int64_t x_stride, const void *y, int64_t y_stride, void *out,
                     int64_t out_stride, int dtype, int64_t M, int64_t H, int64_t N, int64_t r,

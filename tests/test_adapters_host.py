@@ -23,7 +23,8 @@ def xp_add(x=P, xs=64, y=P, ys=32, out=P, os=32, dtype=1, M=4, H=64, N=32, r=8, 
     ({"dtype": 0}, native.XP_EINVAL), ({"dtype": 3}, native.XP_EINVAL),
     ({"M": -1}, native.XP_EINVAL), ({"H": 0}, native.XP_EINVAL), ({"N": 0}, native.XP_EINVAL),
     ({"r": 0}, native.XP_EINVAL), ({"r": 129}, native.XP_ERANGE),
-    ({"slots": 0}, native.XP_EINVAL), ({"M": (1 << 26) + 1}, native.XP_ERANGE),
+    ({"slots": 0}, native.XP_EINVAL), ({"slots": 8193}, native.XP_ERANGE),
+    ({"H": 1 << 31}, native.XP_ERANGE), ({"N": 1 << 31}, native.XP_ERANGE), ({"M": (1 << 26) + 1}, native.XP_ERANGE),
     ({"ids_bytes": 2}, native.XP_EINVAL), ({"xs": -1}, native.XP_EINVAL),
     ({"ys": -1}, native.XP_EINVAL), ({"os": 31}, native.XP_EINVAL),
     ({"adapters_": -1}, native.XP_EINVAL), ({"x": None}, native.XP_EINVAL),
@@ -39,6 +40,7 @@ def test_scratch_size():
     need = native.lib().xp_low_rank_scratch_bytes
     assert need(0, 4) >= 0 and need(1, 4) >= 0
     assert need(-1, 4) == -1 and need(1, 0) == -1 and need((1 << 26) + 1, 4) == -1
+    assert need(1, 8193) == -1
     big = need(1 << 16, 8)
     if big:
         assert xp_add(M=1 << 16, slots=8) == native.XP_EINVAL  # no scratch
@@ -95,9 +97,9 @@ def test_add_low_rank_refusals(any_device, change, words):
 
 
 def test_rank_limit(any_device):
-    with pytest.raises(ValueError, match="rank at most 128"):
+    with pytest.raises(ValueError, match="the rank at most 128"):
         adapters.add_low_rank(**operands(r=129))
-    with pytest.raises(ValueError, match="rank at most 128"):
+    with pytest.raises(ValueError, match="the rank at most 128"):
         adapters.add_low_rank(**operands(r=0))
 
 
@@ -123,9 +125,14 @@ def test_overlap_is_refused(any_device):
 
 def test_columns_of_one_buffer_do_not_overlap():
     wide = torch.zeros((6, 64), dtype=torch.bfloat16)
-    assert not adapters._share(wide[:, :24], wide[:, 24:48])
-    assert not adapters._share(wide[:, 40:], wide[:, :40])
-    assert adapters._share(wide[:, :24], wide[:, 23:48])
-    assert adapters._share(wide[:, 30:50], wide[:, 10:31])
-    assert adapters._share(wide, wide[3:4])
-    assert not adapters._share(wide[:3], wide[3:])
+
+    def share(u, v):
+        return adapters._overlap(u.data_ptr(), u.stride(0), u.shape[1], v.data_ptr(),
+                                 v.stride(0), v.shape[1], u.shape[0])
+
+    assert not share(wide[:, :24], wide[:, 24:48])
+    assert not share(wide[:, 40:], wide[:, :40])
+    assert share(wide[:, :24], wide[:, 23:48])
+    assert share(wide[:, 30:50], wide[:, 10:31])
+    assert share(wide[:3], wide[2:5]) and share(wide, wide)
+    assert not share(wide[:3], wide[3:])

@@ -64,7 +64,7 @@ def test_balance_checks_its_arguments(change, status):
 @pytest.mark.parametrize("change, status", [
     ({"topk": 40}, native.XP_ERANGE), ({"ids": None}, native.XP_EINVAL),
     ({"grad": None}, native.XP_EINVAL), ({"counts": None}, native.XP_EINVAL),
-    ({"tokens": None}, native.XP_EINVAL), ({"logits": None}, native.XP_EINVAL),
+    ({"tokens": None, "valid": P}, native.XP_EINVAL), ({"logits": None}, native.XP_EINVAL),
     ({"E": 0}, native.XP_EINVAL), ({"T": 0}, native.XP_OK),
 ])
 def test_backward_checks_its_arguments(change, status):
@@ -139,8 +139,8 @@ def test_launch_enters_the_tensors_device(monkeypatch):
     seen, current = [], [0]
 
     class Device:
-        def __init__(self, d):
-            self.index = d.index
+        def __init__(self, index):
+            self.index = index
 
         def __enter__(self):
             self.was, current[0] = current[0], self.index
@@ -148,13 +148,9 @@ def test_launch_enters_the_tensors_device(monkeypatch):
         def __exit__(self, *a):
             current[0] = self.was
 
-    class Stream:
-        def __init__(self, d):
-            self.cuda_stream = 1000 + d.index
-
     monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
     monkeypatch.setattr(torch.cuda, "device", Device)
-    monkeypatch.setattr(torch.cuda, "current_stream", Stream)
+    monkeypatch.setattr(native, "_stream", lambda index: 1000 + index)
 
     def fn(x, stream):
         seen.append((x, stream, current[0]))

@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(256, VPL <= 16 ? 4 : (VPL <= 32 ? 2 : 1))
   {
     float s = 0.0f;
     if (balance) {
-      const float n = static_cast<float>(*a.tokens);
+      const float n = static_cast<float>(a.tokens ? *a.tokens : a.T);
       if (n > 0.0f) s = *a.grad_loss * E / n / (n * a.topk);
     }
     for (int e = threadIdx.x; e < E; e += blockDim.x)
@@ -634,7 +634,8 @@ extern "C" int xp_route_backward(const void *logits, int dtype, int64_t T, int64
   if (rc) return rc;
   if (grad_weights && topk > XP_MAX_TOPK) return XP_ERANGE;
   if (T == 0) return XP_OK;
-  if (!logits || !grad || (grad_weights && !ids) || (grad_loss && (!counts || !tokens)))
+  if (!logits || !grad || (grad_weights && !ids) || (grad_loss && !counts) ||
+      (grad_loss && valid && !tokens))
     return XP_EINVAL;
   BackwardArgs a{logits, T, stride, static_cast<int>(E), static_cast<int>(topk), renormalize,
                  valid, ids, grad_weights, counts, tokens,

@@ -20,6 +20,7 @@ import torch
 from vllm_expert_pager import native
 
 _DTYPES = (torch.bfloat16, torch.float16)
+_ID_DTYPES = {torch.int32: 4, torch.int64: 8}
 
 
 @functools.lru_cache(maxsize=1024)
@@ -27,25 +28,14 @@ def _scratch_bytes(rows: int, slots: int) -> int:
     return native.lib().xp_low_rank_scratch_bytes(rows, slots)
 
 
-def _span(t: torch.Tensor) -> tuple[int, int]:
-    """First byte of a 2-d tensor and the byte after its last."""
-    p = t.data_ptr()
-    if not t.numel():
-        return p, p
-    last = (t.shape[0] - 1) * t.stride(0) + t.shape[1]
-    return p, p + last * t.element_size()
-
-
-def _share(u: torch.Tensor, v: torch.Tensor) -> bool:
-    """Whether two row tensors have bytes in common (columns of one buffer may not)."""
-    (u0, u1), (v0, v1) = _span(u), _span(v)
-    if u1 <= v0 or v1 <= u0:
+def _overlap(p: int, ps: int, pw: int, q: int, qs: int, qw: int, rows: int) -> bool:
+    """Whether two operands of ``rows`` rows of 16-bit values have bytes in common: first address,
+    row stride and width of each.  Columns of one buffer that lie apart have none."""
+    if q + 2 * ((rows - 1) * qs + qw) <= p or p + 2 * ((rows - 1) * ps + pw) <= q:
         return False
-    pitch = u.stride(0) * u.element_size()
-    if pitch == v.stride(0) * v.element_size() and pitch > 0:
-        off = (v0 - u0) % pitch  # v's columns, counted from u's, in a row of the buffer
-        width = u.shape[1] * u.element_size()
-        if off >= width and off + v.shape[1] * v.element_size() <= pitch:
+    if ps == qs and ps > 0:
+        off = (q - p) % (2 * ps)  # q's columns, counted from p's, in a row of the buffer
+        if off >= 2 * pw and off + 2 * qw <= 2 * ps:
             return False
     return True
 
@@ -86,12 +76,14 @@ def add_low_rank(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
                          f"{t}, {y.dtype}, {a.dtype}, {b.dtype} and {out.dtype}")
     if not (y.device == a.device == b.device == ids.device == out.device == dev):
         raise ValueError("all operands must be on one device")
-    if H < 1 or N < 1 or S < 1 or not 1 <= r <= native.MAX_RANK:
-        raise ValueError(f"sizes must be at least 1 and the rank at most {native.MAX_RANK}, got "
-                         f"in {H}, out {N}, slots {S}, rank {r}")
+    if (H < 1 or N < 1 or not 1 <= S <= native.MAX_ADAPTER_SLOTS
+            or not 1 <= r <= native.MAX_RANK):
+        raise ValueError(f"sizes must be at least 1, the rank at most {native.MAX_RANK} and the "
+                         f"slots at most {native.MAX_ADAPTER_SLOTS}, got in {H}, out {N}, rank "
+                         f"{r}, slots {S}")
     if M > native.MAX_TOKENS:
         raise ValueError(f"at most {native.MAX_TOKENS} rows are supported, got {M}")
-    if ids.dtype not in (torch.int32, torch.int64):
+    if ids.dtype not in _ID_DTYPES:
         raise ValueError(f"ids must be int32 or int64, got {ids.dtype}")
     if scale is not None and (scale.dtype != torch.float32 or scale.shape != (S,)
                               or scale.device != dev):
@@ -101,24 +93,29 @@ def add_low_rank(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
                                  or slot_map.device != dev):
         raise ValueError(f"slot_map must be an int32 vector on {dev}, got {slot_map.dtype} "
                          f"{list(slot_map.shape)} on {slot_map.device}")
-    if torch.is_grad_enabled() and any(v is not None and v.requires_grad
-                                       for v in (y, x, a, b, scale, out)):
+    if ((x.requires_grad or y.requires_grad or a.requires_grad or b.requires_grad
+         or out.requires_grad or scale is not None and scale.requires_grad)
+            and torch.is_grad_enabled()):
         raise ValueError("add_low_rank has no gradient: call it under torch.no_grad() or on "
                          "detached tensors")
     if not (a.is_contiguous() and b.is_contiguous()):
         raise ValueError("adapter slabs must be contiguous")
-    if out.stride(1) != 1 and N > 1 or out.stride(0) < N and M > 1:
+    (xs, xe), (ys, ye), (os, oe) = x.stride(), y.stride(), out.stride()
+    if oe != 1 and N > 1 or os < N and M > 1:
         raise ValueError("the rows of out must be contiguous and apart")
-    if x.stride(1) != 1:
-        x = x.contiguous()
-    if y.stride(1) != 1:
-        y = y.contiguous()
-    ids = ids.contiguous()
     if M == 0:
         return out
-    if _share(out, x) or (out is not y and _share(out, y)
-                          and (out.data_ptr(), out.stride(0)) != (y.data_ptr(), y.stride(0))):
+    xp, yp, op = x.data_ptr(), y.data_ptr(), out.data_ptr()
+    if _overlap(op, os, N, xp, xs, H, M) or ((op, os) != (yp, ys)
+                                             and _overlap(op, os, N, yp, ys, N, M)):
         raise ValueError("out may be y itself, and may not overlap x or other rows of y")
+    if xe != 1:
+        x = x.contiguous()
+        xp, xs = x.data_ptr(), x.stride(0)
+    if ye != 1:
+        y = y.contiguous()
+        yp, ys = y.data_ptr(), y.stride(0)
+    ids = ids.contiguous()
     if scale is not None:
         scale = scale.contiguous()
     if slot_map is not None:
@@ -126,8 +123,8 @@ def add_low_rank(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     need = _scratch_bytes(M, S)
     scratch = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
     native.launch(dev, "add_low_rank", native.lib().xp_add_low_rank,
-                  x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), out.data_ptr(),
-                  out.stride(0), native.DTYPES[t], M, H, N, r, a.data_ptr(), b.data_ptr(), S,
-                  native.ptr(scale), ids.data_ptr(), ids.element_size(), native.ptr(slot_map),
-                  0 if slot_map is None else slot_map.shape[0], native.ptr(scratch), need)
+                  xp, xs, yp, ys, op, os, native.DTYPES[t], M, H, N, r, a.data_ptr(),
+                  b.data_ptr(), S, native.ptr(scale), ids.data_ptr(), _ID_DTYPES[ids.dtype],
+                  native.ptr(slot_map), 0 if slot_map is None else slot_map.shape[0],
+                  native.ptr(scratch), need)
     return out

@@ -103,6 +103,7 @@ DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_EXPERTS = 4096
 MAX_TOPK = 32
 MAX_RANK = 128
+MAX_ADAPTER_SLOTS = 8192
 MAX_TOKENS = 1 << 26
 
 _lib: ctypes.CDLL | None = None
@@ -144,13 +145,22 @@ def stream_of(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# The same handle without the Stream object around it (2 us less on each call).
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _stream)
+
+
 def launch(device: torch.device, what: str, fn, *args) -> None:
     """Call ``fn(*args, stream)`` on the current stream of ``device``, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream(index))
     if rc != XP_OK:
         check(rc, what)
 

@@ -69,7 +69,9 @@ def _forward(logits, topk, renormalize, valid, balance, given, count_tokens):
     dev = logits.device
     empty = torch.empty
     counts = empty((E,), dtype=torch.int64, device=dev)
-    tokens = empty((1,), dtype=torch.int64, device=dev) if count_tokens else None
+    # Without padding the backward pass knows the number of tokens: all rows.
+    tokens = (empty((1,), dtype=torch.int64, device=dev) if count_tokens and valid is not None
+              else None)
     loss = empty((), dtype=torch.float32, device=dev) if balance else None
     need = _scratch_bytes(T, E)
     scratch = empty((need,), dtype=torch.uint8, device=dev) if need else None
@@ -99,11 +101,11 @@ def _backward(logits, topk, renormalize, valid, ids, grad_weights, counts, token
         grad_weights = grad_weights.contiguous()
     T, E = logits.shape
     grad = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
+    ptr = native.ptr
     native.launch(logits.device, "route_backward", native.lib().xp_route_backward,
                   logits.data_ptr(), native.DTYPES[logits.dtype], T, E, logits.stride(0),
-                  native.ptr(valid), native.ptr(ids), topk, renormalize,
-                  native.ptr(grad_weights), native.ptr(counts), native.ptr(tokens),
-                  native.ptr(grad_loss), grad.data_ptr())
+                  ptr(valid), ptr(ids), topk, renormalize, ptr(grad_weights), ptr(counts),
+                  ptr(tokens), ptr(grad_loss), grad.data_ptr())
     return grad
 
 
