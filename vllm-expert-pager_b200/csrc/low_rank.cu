@@ -25,6 +25,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace xp {
@@ -37,9 +39,9 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kRowsLimit = 512;   // rows_kernel up to here
 constexpr int kGroup = 8;         // rows of a cluster of rows_kernel
-constexpr int kTile = 64;         // rows of a tile
-constexpr int kStages = 4;        // ring of tile_kernel
+constexpr int kTile = 128;        // rows of a tile
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanCtas = 8;      // one cluster
 
 struct LowRankArgs {
   const void *x, *y;
@@ -131,29 +133,93 @@ __device__ __forceinline__ int slot_of_row(const LowRankArgs &a, int64_t m) {
   return s >= 0 && s < a.slots ? static_cast<int>(s) : -1;
 }
 
-// Eight neighbouring values, those from `valid` on as zeros (valid may be <= 0).
+// Eight neighbouring values at any place, those from `valid` on as zeros (valid may
+// be <= 0): the aligned 16-byte words around them (those two that hold at least one
+// of the values), then shifts, which takes a quarter of the loads that single values
+// would.  Two steps, so that several fetches can be under way.
+struct Words {
+  uint4 lo, hi;
+};
+
+template <typename T>
+__device__ __forceinline__ Words fetch_words(const T *p, int64_t valid) {
+  Words w = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  if (valid <= 0) return w;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  const int off = static_cast<int>(at & 15), n = valid < 8 ? static_cast<int>(valid) : 8;
+  const uint4 *word = reinterpret_cast<const uint4 *>(at - off);
+  w.lo = __ldg(word);
+  if (off + 2 * n > 16) w.hi = __ldg(word + 1);
+  return w;
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 join_words(const Words &v, const T *p, int64_t valid) {
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
+  const int n = valid < 0 ? 0 : (valid < 8 ? static_cast<int>(valid) : 8);
+  uint32_t w[8] = {v.lo.x, v.lo.y, v.lo.z, v.lo.w, v.hi.x, v.hi.y, v.hi.z, v.hi.w};
+  if (off & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (off & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  if (off & 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (2 * i + 2 > n) w[i] &= 2 * i + 1 > n ? 0u : 0xffffu;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 template <typename T>
 __device__ __forceinline__ uint4 load8(const T *p, int64_t valid, bool vec) {
   if (vec && valid >= 8) return __ldg(reinterpret_cast<const uint4 *>(p));
-  uint4 q = make_uint4(0, 0, 0, 0);
-  const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < valid) (&q.x)[i >> 1] |= static_cast<uint32_t>(__ldg(h + i)) << (16 * (i & 1));
-  return q;
+  return join_words(fetch_words(p, valid), p, valid);
 }
 
-__device__ __forceinline__ void copy_row(const LowRankArgs &a, int64_t m, int part, int parts) {
-  const uint16_t *y = static_cast<const uint16_t *>(a.y) + m * a.y_stride;
-  uint16_t *out = static_cast<uint16_t *>(a.out) + m * a.out_stride;
-  const int64_t first = static_cast<int64_t>(part) * kThreads + threadIdx.x;
-  const int64_t step = static_cast<int64_t>(parts) * kThreads;
-  if (a.vec_y) {
-    for (int64_t n = first; n < a.N / 8; n += step)
-      reinterpret_cast<uint4 *>(out)[n] = reinterpret_cast<const uint4 *>(y)[n];
-    for (int64_t n = a.N / 8 * 8 + first; n < a.N; n += step) out[n] = y[n];
+// Eight neighbouring values of which `valid` exist, to any place.
+template <typename T>
+__device__ __forceinline__ void put8(T *p, const uint4 &q, int64_t valid, bool vec) {
+  if (vec && valid >= 8) {
+    *reinterpret_cast<uint4 *>(p) = q;
   } else {
-    for (int64_t n = first; n < a.N; n += step) out[n] = y[n];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < valid)
+        reinterpret_cast<uint16_t *>(p)[e] =
+            static_cast<uint16_t>((&q.x)[e >> 1] >> (16 * (e & 1)));
+  }
+}
+
+// out = y for n_rows rows (row(i): the i-th): part `part` of `parts`, by the whole
+// block, four pieces of a thread under way.
+template <typename T, typename Row>
+__device__ __forceinline__ void copy_rows(const LowRankArgs &a, int n_rows, int part, int parts,
+                                          Row row) {
+  const int64_t pieces = (a.N + 7) / 8, all = n_rows * pieces;
+  const int64_t step = static_cast<int64_t>(parts) * blockDim.x;
+  for (int64_t i0 = static_cast<int64_t>(part) * blockDim.x + threadIdx.x; i0 < all;
+       i0 += 4 * step) {
+    uint4 q[4];
+    int64_t m[4], n[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t i = i0 + j * step;
+      if (i < all) {
+        m[j] = row(static_cast<int>(i / pieces));
+        n[j] = i % pieces * 8;
+        q[j] = load8(static_cast<const T *>(a.y) + m[j] * a.y_stride + n[j], a.N - n[j], a.vec_y);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i0 + j * step < all)
+        put8(static_cast<T *>(a.out) + m[j] * a.out_stride + n[j], q[j], a.N - n[j], a.vec_y);
   }
 }
 
@@ -178,7 +244,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
   const int m = blockIdx.x / C, M = static_cast<int>(a.M);
   const int s = slot_of_row(a, m);
   if (s < 0) {
-    if (!a.in_place) copy_row(a, m, rank, C);
+    if (!a.in_place) copy_rows<T>(a, 1, rank, C, [&](int) { return static_cast<int64_t>(m); });
     return;  // every CTA of the cluster
   }
   // The rows of this adapter: a cluster leads where its row is the first of
@@ -322,33 +388,59 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
 
 // ---- long batches ----
 
-// Sorts the rows by slot and cuts each slot's rows into tiles.  The order of a
-// slot's rows is free: a row's result does not depend on its tile.
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ LowRankArgs a) {
-  extern __shared__ int count[];  // [slots + 1]: rows, then the next free place
+// Sorts the rows by slot and cuts each slot's rows into tiles: one cluster, a run of
+// rows for each CTA; the CTAs' counts go through distributed shared memory.  The
+// order of a slot's rows is free: a row's result does not depend on its tile.
+__global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads)
+    plan_kernel(const __grid_constant__ LowRankArgs a) {
+  extern __shared__ int counts[];  // [slots + 1] rows of this CTA; [slots + 1] next free place
   __shared__ int sum_rows[32], sum_tiles[32];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = cluster.block_rank();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int n = a.slots + 1, M = static_cast<int>(a.M);  // the last: rows without an adapter
-  for (int i = tid; i < n; i += kPlanThreads) count[i] = 0;
+  int *place = counts + n;
+  const int per = (M + kPlanCtas - 1) / kPlanCtas, first = min(rank * per, M),
+            last = min(first + per, M);
+  for (int i = tid; i < n; i += kPlanThreads) counts[i] = 0;
   __syncthreads();
-  for (int m0 = warp * 32; m0 < M; m0 += kPlanThreads) {
-    const int m = m0 + lane;
-    int s = -2;
-    if (m < M) {
-      s = slot_of_row(a, m);
-      if (s < 0) s = a.slots;
+  // Four rows of a thread at a time: their ids (and map entries) come together.
+  constexpr int kBatch = 4;
+  auto slots_of = [&](int m0, int (&s)[kBatch]) {
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int m = m0 + j * kPlanThreads + lane;
+      s[j] = -2;
+      if (m < last) {
+        s[j] = slot_of_row(a, m);
+        if (s[j] < 0) s[j] = a.slots;
+      }
     }
-    const unsigned peers = __match_any_sync(kFull, s);
-    if (s >= 0 && lane == __ffs(peers) - 1) atomicAdd(&count[s], __popc(peers));
+  };
+  for (int m0 = first + warp * 32; m0 < last; m0 += kBatch * kPlanThreads) {
+    int s[kBatch];
+    slots_of(m0, s);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const unsigned peers = __match_any_sync(kFull, s[j]);
+      if (s[j] >= 0 && lane == __ffs(peers) - 1) atomicAdd(&counts[s[j]], __popc(peers));
+    }
   }
-  __syncthreads();
-  // Exclusive sums over the slots, a run of slots per thread.
+  cluster.sync();
+  // Exclusive sums over the slots, a run of slots per thread; every CTA has its own.
   const int run = (n + kPlanThreads - 1) / kPlanThreads, i0 = min(tid * run, n),
             i1 = min(i0 + run, n);
   int rows = 0, tiles = 0;
   for (int i = i0; i < i1; ++i) {
-    rows += count[i];
-    if (i < a.slots || !a.in_place) tiles += (count[i] + kTile - 1) / kTile;
+    int all = 0, before = 0;
+#pragma unroll
+    for (int b = 0; b < kPlanCtas; ++b) {
+      if (b == rank) before = all;
+      all += cluster.map_shared_rank(counts, b)[i];
+    }
+    place[i] = before;  // of the slot's rows, those of the CTAs before this one
+    rows += all;
+    if (i < a.slots || !a.in_place) tiles += (all + kTile - 1) / kTile;
   }
   int rows_before = rows, tiles_before = tiles;
 #pragma unroll
@@ -363,29 +455,30 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
   tiles_before -= tiles;
   for (int w = 0; w < warp; ++w) rows_before += sum_rows[w], tiles_before += sum_tiles[w];
   for (int i = i0; i < i1; ++i) {
-    const int rows_here = count[i];
-    count[i] = rows_before;
-    if (i < a.slots || !a.in_place)
-      for (int o = 0; o < rows_here; o += kTile)
+    int all = 0;
+#pragma unroll
+    for (int b = 0; b < kPlanCtas; ++b) all += cluster.map_shared_rank(counts, b)[i];
+    if (rank == 0 && (i < a.slots || !a.in_place))
+      for (int o = 0; o < all; o += kTile)
         a.tiles[tiles_before++] =
-            make_int4(i < a.slots ? i : -1, rows_before + o, min(kTile, rows_here - o), 0);
-    rows_before += rows_here;
+            make_int4(i < a.slots ? i : -1, rows_before + o, min(kTile, all - o), 0);
+    place[i] += rows_before;
+    rows_before += all;
   }
-  if (tid == kPlanThreads - 1) *a.ntiles = tiles_before;
-  __syncthreads();
-  for (int m0 = warp * 32; m0 < M; m0 += kPlanThreads) {
-    const int m = m0 + lane;
-    int s = -2;
-    if (m < M) {
-      s = slot_of_row(a, m);
-      if (s < 0) s = a.slots;
+  if (rank == 0 && tid == kPlanThreads - 1) *a.ntiles = tiles_before;
+  cluster.sync();  // the counts stay until all have read them
+  for (int m0 = first + warp * 32; m0 < last; m0 += kBatch * kPlanThreads) {
+    int s[kBatch];
+    slots_of(m0, s);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const unsigned peers = __match_any_sync(kFull, s[j]);
+      const int leader = __ffs(peers) - 1;
+      int at = 0;
+      if (s[j] >= 0 && lane == leader) at = atomicAdd(&place[s[j]], __popc(peers));
+      at = __shfl_sync(kFull, at, leader) + __popc(peers & lanemask_lt());
+      if (s[j] >= 0) a.perm[at] = m0 + j * kPlanThreads + lane;
     }
-    const unsigned peers = __match_any_sync(kFull, s);
-    int place = 0;
-    const int leader = __ffs(peers) - 1;
-    if (s >= 0 && lane == leader) place = atomicAdd(&count[s], __popc(peers));
-    place = __shfl_sync(kFull, place, leader) + __popc(peers & lanemask_lt());
-    if (s >= 0) a.perm[place] = m;
   }
 }
 
@@ -393,252 +486,552 @@ __device__ __forceinline__ uint32_t smem_addr(const void *p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
+// 16 bytes into shared memory, asynchronously; bytes from `bytes` on are zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
 }
 
-// Eight values into shared memory, those from `valid` on as zeros: asynchronously
-// where 16-byte accesses are allowed.
-template <typename T>
-__device__ __forceinline__ void fetch8(uint32_t dst, const T *src, int64_t valid, bool vec) {
-  if (vec) {
-    const int bytes = valid >= 8 ? 16 : (valid <= 0 ? 0 : static_cast<int>(valid) * 2);
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
-                 : "memory");
-  } else {
-    const uint4 q = load8(src, valid, false);
-    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(q.x), "r"(q.y), "r"(q.z),
-                 "r"(q.w)
-                 : "memory");
+__device__ __forceinline__ void store16(uint32_t dst, const uint4 &q) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(q.x), "r"(q.y), "r"(q.z),
+               "r"(q.w)
+               : "memory");
+}
+
+// mbarriers.  A wait gives up after kWaitNs or when another one of the block has:
+// it then sets *failed.
+constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr int kFreePolls = 256;  // tries before the time is looked at
+
+__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Arrives at the barrier at the same place in another CTA of the cluster.
+__device__ __forceinline__ void bar_arrive_peer(uint32_t bar, int cta) {
+  asm volatile(
+      "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, %1;\n\t"
+      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n\t}" ::"r"(bar),
+      "r"(cta)
+      : "memory");
+}
+
+template <bool kCluster = false>
+__device__ __forceinline__ bool bar_wait(uint32_t bar, int parity, volatile int *failed) {
+  uint64_t since = 0;
+  for (int i = 0;; ++i) {
+    uint32_t done;
+    if constexpr (kCluster)
+      asm volatile(
+          "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], "
+          "%2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(done)
+          : "r"(bar), "r"(parity)
+          : "memory");
+    else
+      asm volatile(
+          "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(done)
+          : "r"(bar), "r"(parity)
+          : "memory");
+    if (done) return true;
+    if (i < kFreePolls) continue;
+    const uint64_t now = global_ns();
+    if (i == kFreePolls) since = now;
+    if (*failed || now - since > kWaitNs) break;
   }
+  *failed = 1;
+  return false;
 }
 
-constexpr int kPitch = 144;  // bytes of a row of 64 values: 16 more, so that 8 rows meet 8 banks
+__device__ __forceinline__ void fence_async_proxy() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
 
+// The barrier completes when the matrix instructions issued so far have.
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                   bar)
+               : "memory");
+}
+
+// Operand in shared memory: rows of 128 bytes along the summed axis, 16-byte pieces
+// exchanged within 8 rows (128-byte swizzle), 1024 bytes from 8 rows to the next 8.
+__device__ __forceinline__ uint64_t operand(uint32_t addr) {
+  return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | (1ull << 16) | (64ull << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+
+// d[128, N] (+)= a[128, 16] b[N, 16]^T, 32-bit sums in tensor memory.
+__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t what,
+                                       bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(what), "r"(static_cast<uint32_t>(add))
+      : "memory");
+}
+
+// This thread's row of tensor memory, 16 columns.
+__device__ __forceinline__ void tc_load16(float (&v)[16], uint32_t addr) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Byte of 16-byte piece `piece` of row `row` in a swizzled block of 128-byte rows.
+__device__ __forceinline__ int swizzled(int row, int piece) {
+  return row * 128 + ((piece ^ (row & 7)) << 4);
+}
+
+constexpr int kOutWarps = 8;                 // half a row of the tile for each thread
+constexpr int kMmaWarp = kOutWarps;          // issues the matrix instructions
+constexpr int kLoadWarps = 4;
+constexpr int kLoaders = kLoadWarps * 32;
+constexpr int kTileThreads = (kOutWarps + 1 + kLoadWarps) * 32;
+constexpr int kStages = 3;
+constexpr int kNBlock = 64;                  // columns of out in a stage
+constexpr int kTmemCols = 256;               // v: 128 at most, then two blocks of out
+constexpr int kTmemOut = 128;
+
+// kRB: blocks of 16 ranks.  kAtoms: 128-byte rows that hold a row of ranks.
 template <int kRB>
 struct TileSmem {
   static constexpr int kR = kRB * 16;
-  static constexpr int kPitchB = kR * 2 + 16;  // bytes of a row of B
-  // A stage holds 64 rows x 64 values of x and kR x 64 of A, or 64 rows of B and 64 x 64 of y.
-  static constexpr int kFirst = kTile * kPitch + kR * kPitch;
-  static constexpr int kSecond = 64 * kPitchB + kTile * kPitch;
-  static constexpr int kStage = kFirst > kSecond ? kFirst : kSecond;
-  static constexpr int kPitchV = kR + 4;  // floats of a row of v
-  static constexpr int kV = kTile * kPitchV * 4;
-  static constexpr int kBytes = kStages * kStage + kV;
+  static constexpr int kAtoms = kR > 64 ? 2 : 1;
+  // A stage holds 128 rows x 64 values of x and kR x 64 of A, or 64 rows of B and 128 x 64 of y.
+  static constexpr int kA = kTile * 128;
+  static constexpr int kY = kAtoms * kNBlock * 128;
+  static constexpr int kFirst = kA + kR * 128, kSecond = kY + kTile * 128;
+  static constexpr int kStage = ((kFirst > kSecond ? kFirst : kSecond) + 1023) / 1024 * 1024;
+  // The high parts of v, then the low parts; before them this CTA's share of v (32-bit).
+  static constexpr int kV = 2 * kAtoms * kTile * 128;
+  static_assert(kR * kTile * 4 <= kV, "a share of v has room where v goes");
+  static constexpr int kBytes = 1024 + kStages * kStage + kV;
 };
 
-template <typename T, int kRB>
-__global__ void __launch_bounds__(kThreads, kRB <= 4 ? 2 : 1)
+// kVec: all rows allow 16-byte accesses (else each operand goes by its own flag; the
+// shifts of odd places need more registers than two CTAs on an SM leave).
+template <typename T, int kRB, bool kVec>
+__global__ void __launch_bounds__(kTileThreads, kVec && kRB <= 4 ? 2 : 1)
     tile_kernel(const __grid_constant__ LowRankArgs a) {
   using S = TileSmem<kRB>;
-  extern __shared__ __align__(16) unsigned char smem[];
+  const bool vec_x = kVec || a.vec_x, vec_a = kVec || a.vec_a, vec_b = kVec || a.vec_b,
+             vec_y = kVec || a.vec_y;
+  extern __shared__ unsigned char raw[];
   __shared__ int64_t rows[kTile];
-  __shared__ float factor[kTile];
-  float *v = reinterpret_cast<float *>(smem + kStages * S::kStage);
+  __shared__ __align__(8) uint64_t bars[3 * kStages + 8];
+  __shared__ float amax[2][kTile];
+  __shared__ uint32_t tmem_at;
+  __shared__ int failed;
 
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), rank = cluster.block_rank();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int wm = warp & 3, wk = warp >> 2;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int tile = blockIdx.x / C;
   if (tile >= *a.ntiles) return;
   const int4 job = a.tiles[tile];
   const int s = job.x, n_rows = job.z;
-  if (s < 0) {
-    for (int i = 0; i < n_rows; ++i) copy_row(a, a.perm[job.y + i], rank, C);
-    return;
-  }
+  unsigned char *smem =
+      raw + ((1024 - (static_cast<uint32_t>(__cvta_generic_to_shared(raw)) & 1023)) & 1023);
+  const uint32_t ring = smem_addr(smem), v_at = ring + kStages * S::kStage;
+  // Stage filled; stage free after the first / the second product; v in tensor
+  // memory; v in shared memory; a block of out in tensor memory, and read from it;
+  // the cluster's shares of v written, and read.
+  const uint32_t full = smem_addr(bars), free1 = full + 8 * kStages, free2 = free1 + 8 * kStages;
+  const uint32_t v_done = free2 + 8 * kStages, v_ready = v_done + 8, out_done = v_ready + 8,
+                 out_read = out_done + 16, shares = out_read + 16, shares_read = shares + 8;
+  volatile int *fail = &failed;
+
   if (tid < kTile) rows[tid] = a.perm[job.y + min(tid, n_rows - 1)];
-  __syncthreads();
+  if (s < 0) {
+    __syncthreads();
+    copy_rows<T>(a, n_rows, rank, C, [&](int i) { return rows[i]; });
+    return;  // every CTA of the cluster
+  }
+  if (tid == 0) {
+    failed = 0;
+    for (int i = 0; i < kStages; ++i) {
+      bar_init(full + 8 * i, kLoaders);
+      bar_init(free1 + 8 * i, 1);
+      bar_init(free2 + 8 * i, kOutWarps);
+    }
+    bar_init(v_done, 1);
+    bar_init(v_ready, kOutWarps * 32);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(out_done + 8 * i, 1);
+      bar_init(out_read + 8 * i, kOutWarps * 32);
+    }
+    bar_init(shares, C);
+    bar_init(shares_read, C);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_addr(&tmem_at)),
+                 "n"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    tc_fence_before();
+  }
+  if (C > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_at;
 
   const T *A = static_cast<const T *>(a.a) + static_cast<int64_t>(s) * a.r * a.H;
   const T *B = static_cast<const T *>(a.b) + static_cast<int64_t>(s) * a.r * a.N;
-  const T *x = static_cast<const T *>(a.x), *y = static_cast<const T *>(a.y);
   // This CTA's blocks of 64 along H and along N.
-  const int kb_all = static_cast<int>((a.H + 63) / 64), nb_all = static_cast<int>((a.N + 63) / 64);
-  const int k0 = static_cast<int>(static_cast<int64_t>(kb_all) * rank / C);
-  const int k1 = static_cast<int>(static_cast<int64_t>(kb_all) * (rank + 1) / C);
-  const int n0 = static_cast<int>(static_cast<int64_t>(nb_all) * rank / C);
-  const int n1 = static_cast<int>(static_cast<int64_t>(nb_all) * (rank + 1) / C);
+  const int64_t kb_all = (a.H + 63) / 64, nb_all = (a.N + kNBlock - 1) / kNBlock;
+  const int k0 = static_cast<int>(kb_all * rank / C), k1 = static_cast<int>(kb_all * (rank + 1) / C);
+  const int n0 = static_cast<int>(nb_all * rank / C), n1 = static_cast<int>(nb_all * (rank + 1) / C);
   const int first = k1 - k0, chunks = first + n1 - n0;
+  const int k_steps = (a.r + 15) / 16;  // of the second product
 
-  auto issue = [&](int c) {
-    if (c < chunks) {
-      const uint32_t at = smem_addr(smem + (c % kStages) * S::kStage);
-      if (c < first) {
-        const int64_t k = static_cast<int64_t>(k0 + c) * 64;
-        for (int i = tid; i < kTile * 8; i += kThreads) {
-          const int row = i >> 3, e = (i & 7) * 8;
-          fetch8(at + row * kPitch + e * 2, x + rows[row] * a.x_stride + k + e, a.H - k - e,
-                 a.vec_x);
-        }
-        for (int i = tid; i < S::kR * 8; i += kThreads) {
-          const int row = i >> 3, e = (i & 7) * 8;
-          fetch8(at + kTile * kPitch + row * kPitch + e * 2,
-                 A + static_cast<int64_t>(min(row, a.r - 1)) * a.H + k + e,
-                 row < a.r ? a.H - k - e : 0, a.vec_a);
-        }
+  if (warp > kMmaWarp) {
+    // Loading: a thread has one 16-byte piece of every 16th row.
+    const int p = tid - (kMmaWarp + 1) * 32, piece = p & 7, row0 = p >> 3;
+    const uint32_t at0 = ring + swizzled(row0, piece);
+    const int mine = (n_rows - row0 + 15) / 16;  // rows of the tile of this thread
+    constexpr int kEach = kTile / 16;
+    auto clip = [](int64_t values) {  // bytes of a piece of which `values` are left
+      return values >= 8 ? 16 : (values <= 0 ? 0 : static_cast<int>(values) * 2);
+    };
+    // Waits until the stage of chunk c is free; its place, 0 after a wait gave up.
+    auto begin = [&](int c) {
+      const int stage = c % kStages, use = c / kStages;
+      if (use > 0) {
+        const int before = (first + kStages - 1 - stage) / kStages;  // uses by the first product
+        const bool ok = c - kStages < first
+                            ? bar_wait(free1 + 8 * stage, (use - 1) & 1, fail)
+                            : bar_wait(free2 + 8 * stage, (use - 1 - before) & 1, fail);
+        if (!ok) return 0u;
+      }
+      return at0 + stage * S::kStage;
+    };
+    auto end = [&](int c, bool async) {
+      const uint32_t bar = full + 8 * (c % kStages);
+      if (async) {
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
       } else {
-        const int64_t n = static_cast<int64_t>(n0 + c - first) * 64;
-        for (int i = tid; i < 64 * kRB * 2; i += kThreads) {
-          const int row = i / (kRB * 2), e = (i % (kRB * 2)) * 8;
-          const bool in = n + row < a.N;
-          fetch8(at + row * S::kPitchB + e * 2, B + (in ? n + row : 0) * a.r + e,
-                 in ? a.r - e : 0, a.vec_b);
-        }
-        for (int i = tid; i < kTile * 8; i += kThreads) {
-          const int row = i >> 3, e = (i & 7) * 8;
-          fetch8(at + 64 * S::kPitchB + row * kPitch + e * 2, y + rows[row] * a.y_stride + n + e,
-                 row < n_rows ? a.N - n - e : 0, a.vec_y);
-        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_async_proxy();
+        bar_arrive(bar);
       }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  auto arrived = [&]() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-    __syncthreads();
-  };
-
-  for (int c = 0; c < kStages - 1; ++c) issue(c);
-
-  // First product: 16 rows a warp, the two halves of the warps take every other
-  // 32 values of a block.
-  float acc[kRB * 2][4];
+    };
+    // Rows at any place, all of a thread's fetches under way at once.
+    auto odd_rows = [&](uint32_t at, const T *src, int64_t stride, int64_t valid) {
+      Words w[kEach];
 #pragma unroll
-  for (int i = 0; i < kRB * 2; ++i)
+      for (int j = 0; j < kEach; ++j)
+        if (j < mine) w[j] = fetch_words(src + rows[row0 + 16 * j] * stride, valid);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-  for (int c = 0; c < first; ++c) {
-    arrived();
-    issue(c + kStages - 1);
-    const uint32_t at = smem_addr(smem + (c % kStages) * S::kStage);
+      for (int j = 0; j < kEach; ++j)
+        if (j < mine)
+          store16(at + j * 2048, join_words(w[j], src + rows[row0 + 16 * j] * stride, valid));
+    };
+    auto odd_weights = [&](uint32_t at, const T *w0, int64_t stride, int64_t left, int64_t valid,
+                           auto count) {
+      constexpr int kCount = decltype(count)::value;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k = wk * 32 + h * 16;
-      uint32_t p[4];
-      ldmatrix4(p, at + (wm * 16 + (lane & 15)) * kPitch + (k + (lane >> 4) * 8) * 2);
+      for (int j0 = 0; j0 < kCount; j0 += 4) {
+        Words w[4];
 #pragma unroll
-      for (int i = 0; i < kRB; ++i) {
-        uint32_t q[4];  // ranks 16 i .. 16 i + 15: two column blocks of an instruction
-        ldmatrix4(q, at + kTile * kPitch + (i * 16 + (lane >> 4) * 8 + (lane & 7)) * kPitch +
-                         (k + ((lane >> 3) & 1) * 8) * 2);
-        Half<T>::mma(acc[2 * i], p[0], p[1], p[2], p[3], q[0], q[1]);
-        Half<T>::mma(acc[2 * i + 1], p[0], p[1], p[2], p[3], q[2], q[3]);
+        for (int j = 0; j < 4; ++j)
+          if (j0 + j < kCount)
+            w[j] = fetch_words(w0 + (j0 + j) * 16 * stride, 16 * (j0 + j) < left ? valid : 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j0 + j < kCount)
+            store16(at + (j0 + j) * 2048, join_words(w[j], w0 + (j0 + j) * 16 * stride,
+                                                     16 * (j0 + j) < left ? valid : 0));
       }
-    }
-  }
-  // v of this CTA's share of H, the second half of the warps onto the first.
+    };
+
+    bool ok = true;
+    {
+      const T *src[kEach];
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    if (wk == half) {
+      for (int j = 0; j < kEach; ++j)
+        src[j] = static_cast<const T *>(a.x) + (j < mine ? rows[row0 + 16 * j] : 0) * a.x_stride +
+                 static_cast<int64_t>(k0) * 64 + piece * 8;
+      const T *w = A + row0 * a.H + static_cast<int64_t>(k0) * 64 + piece * 8;
+      int64_t left = a.H - static_cast<int64_t>(k0) * 64 - piece * 8;
+      const int ranks = a.r - row0;  // rows of A from this thread's first on
+      for (int c = 0; c < first; ++c, w += 64, left -= 64) {
+        const uint32_t at = begin(c);
+        if (!at) {
+          ok = false;
+          break;
+        }
+        if (vec_x) {
+          const int bytes = clip(left);
 #pragma unroll
-      for (int i = 0; i < kRB * 2; ++i) {
-        float *p = v + (wm * 16 + g) * S::kPitchV + i * 8 + 2 * t, *q = p + 8 * S::kPitchV;
-        if (half == 0) {
-          p[0] = acc[i][0], p[1] = acc[i][1], q[0] = acc[i][2], q[1] = acc[i][3];
+          for (int j = 0; j < kEach; ++j) {
+            if (j < mine) copy16(at + j * 2048, src[j], bytes);
+            src[j] += 64;
+          }
         } else {
-          p[0] += acc[i][0], p[1] += acc[i][1], q[0] += acc[i][2], q[1] += acc[i][3];
+          odd_rows(at, static_cast<const T *>(a.x) + static_cast<int64_t>(k0 + c) * 64 + piece * 8,
+                   a.x_stride, left);
         }
+        if (vec_a) {
+          const int bytes = clip(left);
+#pragma unroll
+          for (int j = 0; j < kRB; ++j)
+            copy16(at + S::kA + j * 2048, 16 * j < ranks ? w + j * 16 * a.H : A,
+                   16 * j < ranks ? bytes : 0);
+        } else {
+          odd_weights(at + S::kA, w, a.H, ranks, left, std::integral_constant<int, kRB>());
+        }
+        end(c, vec_x && vec_a);
       }
     }
-    __syncthreads();
-  }
-  const float scale = a.scale ? a.scale[s] : 1.0f;
-  {
-    // Four lanes a row: the sum over the cluster, the scale and the row's range.
-    const int row = tid >> 2, part = tid & 3;
-    float *p = v + row * S::kPitchV;
-    float u[S::kR / 4], amax = 0.0f;
-    if (C > 1) cluster.sync();
+    if (ok) {
+      const T *src[kEach];
 #pragma unroll
-    for (int i = 0; i < S::kR / 4; ++i) u[i] = 0.0f;
-    for (int b = 0; b < C; ++b) {
-      const float *q = (C > 1 ? cluster.map_shared_rank(v, b) : v) + row * S::kPitchV;
+      for (int j = 0; j < kEach; ++j)
+        src[j] = static_cast<const T *>(a.y) + (j < mine ? rows[row0 + 16 * j] : 0) * a.y_stride +
+                 static_cast<int64_t>(n0) * kNBlock + piece * 8;
+      for (int c = first; c < chunks; ++c) {
+        const uint32_t at = begin(c);
+        if (!at) break;
+        const int64_t n = static_cast<int64_t>(n0 + c - first) * kNBlock;
 #pragma unroll
-      for (int i = 0; i < S::kR / 4; ++i) u[i] += q[i * 4 + part];
-    }
-    if (C > 1) cluster.sync();  // all shares are read; now they may be overwritten
-    float f = 1.0f;
+        for (int q = 0; q < S::kAtoms; ++q) {
+          const int e = q * 64 + piece * 8;
+          if (e >= S::kR) continue;
+          const T *w = B + (n + row0) * a.r + e;
+          const int64_t left = a.N - n - row0;
+          if (vec_b) {
+            const int bytes = clip(a.r - e);
 #pragma unroll
-    for (int i = 0; i < S::kR / 4; ++i) u[i] *= scale, amax = fmaxf(amax, fabsf(u[i]));
-    if constexpr (Half<T>::kNarrowRange) {
-      amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 2));
-      f = range_factor(amax);
-    }
+            for (int j = 0; j < kNBlock / 16; ++j)
+              copy16(at + q * kNBlock * 128 + j * 2048, 16 * j < left ? w + j * 16 * a.r : B,
+                     16 * j < left ? bytes : 0);
+          } else {
+            odd_weights(at + q * kNBlock * 128, w, a.r, left, a.r - e,
+                        std::integral_constant<int, kNBlock / 16>());
+          }
+        }
+        const int64_t left = a.N - n - piece * 8;
+        if (vec_y) {
+          const int bytes = clip(left);
 #pragma unroll
-    for (int i = 0; i < S::kR / 4; ++i) p[i * 4 + part] = u[i] * f;
-    if (part == 0) factor[row] = 1.0f / f;
-  }
-  __syncthreads();
-
-  // Second product: v as the row operand, in two parts.
-  uint32_t hi[kRB][4], lo[kRB][4];
-#pragma unroll
-  for (int i = 0; i < kRB; ++i) {
-    const float *p = v + (wm * 16 + g) * S::kPitchV + i * 16 + 2 * t, *q = p + 8 * S::kPitchV;
-    split<T>(p[0], p[1], &hi[i][0], &lo[i][0]);
-    split<T>(q[0], q[1], &hi[i][1], &lo[i][1]);
-    split<T>(p[8], p[9], &hi[i][2], &lo[i][2]);
-    split<T>(q[8], q[9], &hi[i][3], &lo[i][3]);
-  }
-  const float f0 = factor[wm * 16 + g], f1 = factor[wm * 16 + g + 8];
-  T *out = static_cast<T *>(a.out);
-  for (int c = first; c < chunks; ++c) {
-    arrived();
-    issue(c + kStages - 1);
-    unsigned char *stage = smem + (c % kStages) * S::kStage;
-    const uint32_t at = smem_addr(stage);
-    const int64_t n = static_cast<int64_t>(n0 + c - first) * 64 + wk * 32;
-    float d[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) d[i][j] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kRB; ++i) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        uint32_t q[4];
-        ldmatrix4(q, at + (wk * 32 + j * 16 + (lane >> 4) * 8 + (lane & 7)) * S::kPitchB +
-                         (i * 16 + ((lane >> 3) & 1) * 8) * 2);
-        Half<T>::mma(d[2 * j], hi[i][0], hi[i][1], hi[i][2], hi[i][3], q[0], q[1]);
-        Half<T>::mma(d[2 * j + 1], hi[i][0], hi[i][1], hi[i][2], hi[i][3], q[2], q[3]);
-        Half<T>::mma(d[2 * j], lo[i][0], lo[i][1], lo[i][2], lo[i][3], q[0], q[1]);
-        Half<T>::mma(d[2 * j + 1], lo[i][0], lo[i][1], lo[i][2], lo[i][3], q[2], q[3]);
+          for (int j = 0; j < kEach; ++j) {
+            if (j < mine) copy16(at + S::kY + j * 2048, src[j], bytes);
+            src[j] += kNBlock;
+          }
+        } else {
+          odd_rows(at + S::kY, static_cast<const T *>(a.y) + n + piece * 8, a.y_stride, left);
+        }
+        end(c, vec_b && vec_y);
       }
     }
-    // y + update in place of y in the stage, by the warp whose 16 x 32 values they
-    // are; then whole 16-byte pieces of out.
-    unsigned char *ys = stage + 64 * S::kPitchB + wm * 16 * kPitch + wk * 64;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      constexpr uint32_t kType = Half<T>::kNarrowRange ? 0u : (1u << 7) | (1u << 10);
+      constexpr uint32_t kWhat = (1u << 4) | kType | (8u << 24);  // 32-bit sums, 128 rows
+      constexpr uint32_t kWhat1 = kWhat | (static_cast<uint32_t>(S::kR / 8) << 17);
+      constexpr uint32_t kWhat2 = kWhat | (static_cast<uint32_t>(kNBlock / 8) << 17);
+      bool ok = true;
+      for (int c = 0; c < first && ok; ++c) {
+        const int stage = c % kStages;
+        ok = bar_wait(full + 8 * stage, (c / kStages) & 1, fail);
+        if (!ok) break;
+        fence_async_proxy();
+        tc_fence_after();
+        const uint32_t at = ring + stage * S::kStage;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t *p = reinterpret_cast<uint32_t *>(ys + g * kPitch + i * 16 + 4 * t);
-      uint32_t *q = reinterpret_cast<uint32_t *>(ys + (g + 8) * kPitch + i * 16 + 4 * t);
-      const float2 u = Half<T>::unpack(*p), w = Half<T>::unpack(*q);
-      *p = Half<T>::pack(u.x + d[i][0] * f0, u.y + d[i][1] * f0);
-      *q = Half<T>::pack(w.x + d[i][2] * f1, w.y + d[i][3] * f1);
+        for (int i = 0; i < 4; ++i)
+          tc_mma(tmem, operand(at + 32 * i), operand(at + S::kA + 32 * i), kWhat1, c > 0 || i > 0);
+        tc_commit(free1 + 8 * stage);
+      }
+      if (ok && first > 0) tc_commit(v_done);
+      if (ok && first == 0) bar_arrive(v_done);
+      ok = ok && bar_wait(v_ready, 0, fail);
+      for (int c = first; c < chunks && ok; ++c) {
+        const int stage = c % kStages, i = c - first, half = i & 1;
+        ok = bar_wait(full + 8 * stage, (c / kStages) & 1, fail) &&
+             (i < 2 || bar_wait(out_read + 8 * half, (i / 2 - 1) & 1, fail));
+        if (!ok) break;
+        fence_async_proxy();
+        tc_fence_after();
+        const uint32_t at = ring + stage * S::kStage, d = tmem + kTmemOut + half * kNBlock;
+        for (int part = 0; part < 2; ++part)
+          for (int j = 0; j < k_steps; ++j)
+            tc_mma(d,
+                   operand(v_at + (part * S::kAtoms + j / 4) * kTile * 128 + 32 * (j % 4)),
+                   operand(at + (j / 4) * kNBlock * 128 + 32 * (j % 4)), kWhat2, part + j > 0);
+        tc_commit(out_done + 8 * half);
+      }
     }
     __syncwarp();
+  } else {
+    // Half a row of the tile for each thread (a warp reaches the 32 rows of tensor
+    // memory that its number gives).
+    const int row = tid & 127, side = warp >> 2;
+    const uint32_t my_tmem = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const float scale = a.scale ? a.scale[s] : 1.0f;
+    bool ok = __all_sync(kFull, bar_wait(v_done, 0, fail));
+    tc_fence_after();
+    constexpr int kMine = (kRB + 1) / 2;  // blocks of 16 ranks: every other one is this side's
+    float u[kMine][16];
 #pragma unroll
-    for (int i = lane; i < 64; i += 32) {
-      const int row = i >> 2, e = (i & 3) * 8;
-      if (wm * 16 + row >= n_rows) continue;
-      const int64_t at_n = n + e;
-      T *o = out + rows[wm * 16 + row] * a.out_stride + at_n;
-      const unsigned char *p = ys + row * kPitch + e * 2;
-      if (a.vec_y && at_n + 8 <= a.N) {
-        *reinterpret_cast<uint4 *>(o) = *reinterpret_cast<const uint4 *>(p);
-      } else {
-        for (int j = 0; j < 8 && at_n + j < a.N; ++j) o[j] = reinterpret_cast<const T *>(p)[j];
+    for (int i = 0; i < kMine; ++i) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) u[i][j] = 0.0f;
+      if (ok && first > 0 && 2 * i + side < kRB) tc_load16(u[i], my_tmem + (2 * i + side) * 16);
+    }
+    if (C > 1) {
+      // The cluster's shares of v, added in the order of its CTAs.  They lie where v
+      // will, which is written when all have read them.
+      float *share = reinterpret_cast<float *>(smem + kStages * S::kStage);
+#pragma unroll
+      for (int i = 0; i < kMine; ++i)
+        if (2 * i + side < kRB) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            share[((2 * i + side) * 16 + j) * kTile + row] = u[i][j];
+            u[i][j] = 0.0f;
+          }
+        }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (ok && tid < C) {
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+        bar_arrive_peer(shares, tid);
       }
+      ok = __all_sync(kFull, ok && bar_wait<true>(shares, 0, fail));
+      if (ok) {
+        for (int b = 0; b < C; ++b) {
+          const float *q = cluster.map_shared_rank(share, b) + row;
+#pragma unroll
+          for (int i = 0; i < kMine; ++i)
+            if (2 * i + side < kRB) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) u[i][j] += q[((2 * i + side) * 16 + j) * kTile];
+            }
+        }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (ok && tid < C) bar_arrive_peer(shares_read, tid);
+      ok = __all_sync(kFull, ok && bar_wait<true>(shares_read, 0, fail));
+    }
+    float f = 1.0f;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) u[i][j] *= scale;
+    if constexpr (Half<T>::kNarrowRange) {
+      float most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(u[i][j]));
+      amax[side][row] = most;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      f = range_factor(fmaxf(amax[0][row], amax[1][row]));
+    }
+    const float back = 1.0f / f;
+    if (ok) {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        if (2 * i + side >= kRB) continue;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            split<T>(u[i][h * 8 + 2 * j] * f, u[i][h * 8 + 2 * j + 1] * f, &hi[j], &lo[j]);
+          const int e = 2 * (2 * i + side) + h;  // 16-byte piece of the row
+          const uint32_t at = v_at + (e / 8) * kTile * 128 + swizzled(row, e % 8);
+          store16(at, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+          store16(at + S::kAtoms * kTile * 128, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+        }
+      }
+      fence_async_proxy();
+      tc_fence_before();
+      bar_arrive(v_ready);
+    }
+    for (int c = first; c < chunks && ok; ++c) {
+      const int stage = c % kStages, i = c - first, half = i & 1;
+      ok = __all_sync(kFull, bar_wait(out_done + 8 * half, (i / 2) & 1, fail) &&
+                                 bar_wait(full + 8 * stage, (c / kStages) & 1, fail));
+      if (!ok) break;
+      tc_fence_after();
+      unsigned char *ys = smem + stage * S::kStage + S::kY;
+      // y + update in place of y in the stage, then whole 16-byte pieces of out.
+#pragma unroll
+      for (int j = 2 * side; j < 2 * side + 2; ++j) {
+        float d[16];
+        tc_load16(d, my_tmem + kTmemOut + half * kNBlock + j * 16);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint4 *p = reinterpret_cast<uint4 *>(ys + swizzled(row, 2 * j + h));
+          uint4 q = *p;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 w = Half<T>::unpack((&q.x)[e]);
+            (&q.x)[e] = Half<T>::pack(w.x + d[h * 8 + 2 * e] * back,
+                                      w.y + d[h * 8 + 2 * e + 1] * back);
+          }
+          *p = q;
+        }
+      }
+      tc_fence_before();
+      bar_arrive(out_read + 8 * half);
+      __syncwarp();
+      const int piece = side * 4 + (lane & 3);
+      const int64_t n = static_cast<int64_t>(n0 + i) * kNBlock + piece * 8;
+#pragma unroll
+      for (int q0 = 0; q0 < 4; ++q0) {
+        const int r = (warp & 3) * 32 + q0 * 8 + (lane >> 2);
+        if (r >= n_rows) break;
+        put8(static_cast<T *>(a.out) + rows[r] * a.out_stride + n,
+             *reinterpret_cast<const uint4 *>(ys + swizzled(r, piece)), a.N - n, vec_y);
+      }
+      __syncwarp();
+      if (lane == 0) bar_arrive(free2 + 8 * stage);
     }
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  tc_fence_before();
+  if (C > 1)
+    cluster.sync();  // a CTA's barriers stay until the cluster has used them
+  else
+    __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "n"(kTmemCols));
+  }
+  if (failed) {  // a wait gave up: the rows must not pass for results
+    for (int i = 0; i < n_rows; ++i)
+      for (int64_t n = static_cast<int64_t>(n0) * kNBlock + tid;
+           n < min(a.N, static_cast<int64_t>(n1) * kNBlock); n += kTileThreads)
+        narrow(static_cast<T *>(a.out) + rows[i] * a.out_stride + n, NAN);
+  }
 }
 
 int set_smem(const void *fn, int bytes) {
@@ -647,13 +1040,13 @@ int set_smem(const void *fn, int bytes) {
   return err == cudaSuccess ? XP_OK : static_cast<int>(err);
 }
 
-int launch(const void *fn, unsigned ctas, unsigned cluster, int smem, const LowRankArgs &a,
-           cudaStream_t s) {
+int launch(const void *fn, unsigned ctas, unsigned cluster, int threads, int smem,
+           const LowRankArgs &a, cudaStream_t s) {
   int rc = set_smem(fn, smem);
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas * cluster);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -682,18 +1075,22 @@ template <typename T, int kRB>
 int run_sized(LowRankArgs &a, cudaStream_t s) {
   if (a.M <= kRowsLimit) {
     const unsigned cluster = a.M <= 16 ? 8 : 4;
-    return launch((const void *)rows_kernel<T, kRB>, static_cast<unsigned>(a.M), cluster, 0, a, s);
+    return launch((const void *)rows_kernel<T, kRB>, static_cast<unsigned>(a.M), cluster, kThreads, 0, a,
+                  s);
   }
-  const int bytes = 4 * (a.slots + 1);
+  const int bytes = 8 * (a.slots + 1);
   int rc = set_smem((const void *)plan_kernel, bytes);
   if (rc) return rc;
-  plan_kernel<<<1, kPlanThreads, bytes, s>>>(a);
+  plan_kernel<<<kPlanCtas, kPlanThreads, bytes, s>>>(a);
   rc = launch_status();
   if (rc) return rc;
   const int64_t tiles = most_tiles(a.M, a.slots);
   const int64_t full = (a.M + kTile - 1) / kTile;  // tiles of a batch with few adapters
-  const unsigned cluster = full <= 40 ? 4 : (full <= 148 ? 2 : 1);
-  return launch((const void *)tile_kernel<T, kRB>, static_cast<unsigned>(tiles), cluster,
+  const unsigned cluster = full <= 18 ? 8 : (full <= 37 ? 4 : (full <= 148 ? 2 : 1));
+  const void *fn = a.vec_x && a.vec_a && a.vec_b && a.vec_y
+                       ? (const void *)tile_kernel<T, kRB, true>
+                       : (const void *)tile_kernel<T, kRB, false>;
+  return launch(fn, static_cast<unsigned>(tiles), cluster, kTileThreads,
                 TileSmem<kRB>::kBytes, a, s);
 }
 
