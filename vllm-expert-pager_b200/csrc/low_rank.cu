@@ -25,6 +25,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -39,6 +40,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kRowsLimit = 512;   // rows_kernel up to here
 constexpr int kGroup = 8;         // rows of a cluster of rows_kernel
+constexpr int kRowStages = 3;     // its ring
 constexpr int kTile = 128;        // rows of a tile
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanCtas = 8;      // one cluster
@@ -57,6 +59,7 @@ struct LowRankArgs {
   int64_t adapters;
   int vec_x, vec_a, vec_b, vec_y;  // 16-byte accesses to x, A, B, and y with out
   int in_place;
+  int cluster_log2;  // CTAs of a cluster
   // The plan of tile_kernel.
   int32_t *perm;   // [M] rows by slot
   int4 *tiles;     // (slot, first place in perm, rows, -)
@@ -223,167 +226,346 @@ __device__ __forceinline__ void copy_rows(const LowRankArgs &a, int n_rows, int 
   }
 }
 
+__device__ __forceinline__ uint32_t smem_addr(const void *p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+// 16 bytes into shared memory, asynchronously; bytes from `bytes` on are zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+
+__device__ __forceinline__ void store16(uint32_t dst, const uint4 &q) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(q.x), "r"(q.y), "r"(q.z),
+               "r"(q.w)
+               : "memory");
+}
+
 // ---- short batches ----
 
-// kRB: blocks of 16 ranks.
-template <typename T, int kRB>
-__global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ LowRankArgs a) {
-  constexpr int kR = kRB * 16;
-  __shared__ float red[kWarps][kR * kGroup];
-  __shared__ float part[kR * kGroup];   // [rank][row]: this CTA's share of v
-  __shared__ float vf[kR * kGroup];     // [rank][row]: v
-  __shared__ float factor[kGroup];
-  __shared__ __align__(16) uint16_t vhi[kGroup][kR + 24], vlo[kGroup][kR + 24];
-  __shared__ uint32_t same[kRowsLimit / 32];
-  __shared__ int rows[kGroup];
-  __shared__ int nrows;
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
 
+__device__ __forceinline__ void ldmatrix2(uint32_t (&r)[2], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];"
+               : "=r"(r[0]), "=r"(r[1])
+               : "r"(addr));
+}
+
+// Pitches are 16 bytes longer than the rows, so that eight rows' 16-byte pieces
+// lie in different banks.
+template <int kRB>
+struct RowsSmem {
+  static constexpr int kR = kRB * 16;
+  static constexpr int kK = kRB <= 2 ? 256 : 8192 / kR;  // values of a row of A (and x) in a stage
+  static constexpr int kN = (kRB <= 2 ? 4096 : 8192) / kR;  // rows of B in a stage, columns of y
+  static constexpr int kPitchA = kK * 2 + 16, kPitchB = kR * 2 + 16, kPitchY = kN * 2 + 16;
+  static constexpr int kFirst = (kR + kGroup) * kPitchA;
+  static constexpr int kSecond = kN * kPitchB + kGroup * kPitchY;
+  static constexpr int kStage = kFirst > kSecond ? kFirst : kSecond;
+  static constexpr int kBytes = kRowStages * kStage;
+};
+
+// kRB: blocks of 16 ranks.  kVec: all rows allow 16-byte accesses.
+template <typename T, int kRB, bool kVec>
+__global__ void __launch_bounds__(kThreads, kVec && kRB <= 4 ? 3 : 2)
+    rows_kernel(const __grid_constant__ LowRankArgs a) {
+  using S = RowsSmem<kRB>;
+  constexpr int kR = S::kR, kParts = kWarps / kRB;  // warps that share a block of ranks
+  extern __shared__ __align__(128) unsigned char smem[];
+  constexpr int kPitchV = kR + 4;
+  __shared__ __align__(8) float red[kParts][kGroup * kPitchV];
+  __shared__ __align__(8) float part[kGroup * kPitchV];  // [row][rank]: this CTA's share of v
+  __shared__ float factor[kGroup];
+  __shared__ __align__(16) uint16_t vhi[kGroup][kR + 8], vlo[kGroup][kR + 8];
+  __shared__ __align__(16) int slot[kRowsLimit];
+  __shared__ uint16_t order[kRowsLimit], items[kRowsLimit];
+  __shared__ int found[2];
+  __shared__ int rows[kGroup];
+
+  const bool vec_x = kVec || a.vec_x, vec_a = kVec || a.vec_a, vec_b = kVec || a.vec_b,
+             vec_y = kVec || a.vec_y;
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = cluster.num_blocks(), rank = cluster.block_rank();
+  const int log2c = a.cluster_log2, C = 1 << log2c;
+  const int rank = blockIdx.x & (C - 1), me = blockIdx.x >> log2c, clusters = gridDim.x >> log2c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int m = blockIdx.x / C, M = static_cast<int>(a.M);
-  const int s = slot_of_row(a, m);
-  if (s < 0) {
-    if (!a.in_place) copy_rows<T>(a, 1, rank, C, [&](int) { return static_cast<int64_t>(m); });
-    return;  // every CTA of the cluster
-  }
-  // The rows of this adapter: a cluster leads where its row is the first of
-  // every eight, and takes these eight.
-  for (int w = warp; w < (M + 31) / 32; w += kWarps) {
-    const int j = w * 32 + lane;
-    const uint32_t b = __ballot_sync(kFull, j < M && slot_of_row(a, j) == s);
-    if (lane == 0) same[w] = b;
+  const int M = static_cast<int>(a.M);
+
+  // The items of the batch: eight rows of an adapter at a time, each at the first
+  // of them, then the rows without an adapter.  Every cluster finds them all (one
+  // warp, 32 rows at a time, with the slots' rows so far in the ring) and takes
+  // every so many-th.
+  uint16_t *seen = reinterpret_cast<uint16_t *>(smem);
+  for (int m0 = warp * 32; m0 < M; m0 += kThreads) {
+    const int m = m0 + lane, s = m < M ? slot_of_row(a, m) : -2;
+    const unsigned peers = __match_any_sync(kFull, s);
+    if (m < M) slot[m] = s;
+    if (s >= 0) {  // the rows of the 32 before this one, and whether it is their last
+      order[m] = static_cast<uint16_t>(__popc(peers & lanemask_lt()) | (peers >> lane == 1) << 15);
+      seen[s] = 0;
+    }
   }
   __syncthreads();
   if (warp == 0) {
-    const int words = (M + 31) / 32;
-    uint32_t w = lane < words ? same[lane] : 0;
-    int before = __popc(w);  // set bits of the words before this lane's
+    int leads = 0, alone = 0;
+    constexpr int kAhead = 4;  // words of rows whose slots are read at once
+    for (int m0 = 0; m0 < M; m0 += 32 * kAhead) {
+      int s[kAhead], o[kAhead];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(kFull, before, o);
-      if (lane >= o) before += u;
+      for (int j = 0; j < kAhead; ++j) {
+        const int m = m0 + 32 * j + lane;
+        s[j] = m < M ? slot[m] : -2;
+        o[j] = m < M ? order[m] : 0;
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int m = m0 + 32 * j + lane;
+        int n = 0;  // rows of the same adapter before this one
+        if (s[j] >= 0) {
+          n = (o[j] & 0x7fff) + seen[s[j]];
+          order[m] = static_cast<uint16_t>(n);
+        }
+        __syncwarp();
+        if (s[j] >= 0 && o[j] >> 15) seen[s[j]] = static_cast<uint16_t>(n + 1);
+        const unsigned lead = __ballot_sync(kFull, s[j] >= 0 && n % kGroup == 0);
+        const unsigned none = __ballot_sync(kFull, s[j] == -1 && !a.in_place);
+        if (lead >> lane & 1)
+          items[leads + __popc(lead & lanemask_lt())] = static_cast<uint16_t>(m);
+        if (none >> lane & 1)  // from the end
+          items[kRowsLimit - 1 - alone - __popc(none & lanemask_lt())] = static_cast<uint16_t>(m);
+        leads += __popc(lead);
+        alone += __popc(none);
+        __syncwarp();
+      }
     }
-    const int total = __shfl_sync(kFull, before, 31);
-    before -= __popc(w);
-    const int mine = __shfl_sync(kFull, before + __popc(w & ((1u << (m & 31)) - 1)), m >> 5);
-    if (lane == 0) nrows = mine % kGroup ? 0 : min(kGroup, total - mine);
-    for (; w; w &= w - 1, ++before)
-      if (before >= mine && before < mine + kGroup) rows[before - mine] = lane * 32 + __ffs(w) - 1;
+    if (lane == 0) found[0] = leads, found[1] = alone;
   }
   __syncthreads();
-  const int n_rows = nrows;
-  if (n_rows == 0) return;  // every CTA of the cluster
+  const int leads = found[0], n_items = leads + found[1];
 
-  const T *A = static_cast<const T *>(a.a) + static_cast<int64_t>(s) * a.r * a.H;
-  const T *B = static_cast<const T *>(a.b) + static_cast<int64_t>(s) * a.r * a.N;
-  const int units = C * kWarps, unit = rank * kWarps + warp;
-  const int64_t nblocks = (a.N + 15) / 16;
-  // The second product's weights come on their way while the first one runs.
-  for (int64_t nb = unit; nb < nblocks; nb += units) {
-    const char *p = reinterpret_cast<const char *>(B + nb * 16 * a.r);
-    const int64_t bytes = min(static_cast<int64_t>(16), a.N - nb * 16) * a.r * 2;
-    for (int64_t o = lane * 128; o < bytes; o += 32 * 128)
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(p + o));
-  }
+  const uint32_t ring = smem_addr(smem);
+  // This CTA's part of H and of N, in stages.
+  const uint32_t kb = static_cast<uint32_t>((a.H + 63) / 64);
+  const uint32_t nb = static_cast<uint32_t>((a.N + 15) / 16);
+  const int64_t k0 = static_cast<int64_t>(kb * rank >> log2c) * 64;
+  const int64_t k1 = min(a.H, static_cast<int64_t>(kb * (rank + 1) >> log2c) * 64);
+  const int64_t n0 = static_cast<int64_t>(nb * rank >> log2c) * 16;
+  const int64_t n1 = min(a.N, static_cast<int64_t>(nb * (rank + 1) >> log2c) * 16);
+  const int first = static_cast<int>((k1 - k0 + S::kK - 1) / S::kK);
+  const int chunks = first + static_cast<int>((n1 - n0 + S::kN - 1) / S::kN);
+  // A thread's 16-byte pieces of a stage: a place along the rows, and every so
+  // many-th row.
+  constexpr int kPieces1 = S::kK / 8, kStep1 = kThreads / kPieces1;
+  constexpr int kPieces2 = kRB * 2, kStep2 = kThreads / kPieces2;
+  constexpr int kPiecesY = S::kN / 8;
+  const int e1 = tid % kPieces1 * 8, row1 = tid / kPieces1;
+  const int e2 = tid % kPieces2 * 8, row2 = tid / kPieces2;
+  const int ey = tid % kPiecesY * 8, rowy = tid / kPiecesY;
+  bool again = false;
 
-  // v^T[rank, row]: weights as the 16 rows of an instruction, rows as its columns.
-  // A lane's 16 bytes of a weight row are k = 8t .. 8t+7 of a block of 32; rows
-  // use the same order, so the sum over k is the same one.
-  float c[kRB][4];
+  for (int item = me; item < n_items; item += clusters) {
+    const int m = items[item < leads ? item : kRowsLimit - 1 - (item - leads)], s = slot[m];
+    if (s < 0) {
+      copy_rows<T>(a, 1, rank, C, [&](int) { return static_cast<int64_t>(m); });
+      continue;  // every CTA of the cluster
+    }
+    if (again) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    again = true;
+    int n_rows = 0;
+    for (int j0 = m & ~31; j0 < M; j0 += kThreads) {
+      const int j = j0 + tid;
+      const int n = j < M && slot[j] == s ? order[j] - order[m] : -1;
+      const bool in = n >= 0 && n < kGroup;
+      if (in) rows[n] = j;
+      n_rows += __syncthreads_count(in);
+    }
+
+    const T *A = static_cast<const T *>(a.a) + static_cast<int64_t>(s) * a.r * a.H;
+    const T *B = static_cast<const T *>(a.b) + static_cast<int64_t>(s) * a.r * a.N;
+    const T *xr = static_cast<const T *>(a.x) + rows[min(row1, n_rows - 1)] * a.x_stride + e1;
+    const T *yr = static_cast<const T *>(a.y) + rows[min(rowy, n_rows - 1)] * a.y_stride + ey;
+    auto clip = [](int64_t values) {
+      return values >= 8 ? 16 : (values <= 0 ? 0 : static_cast<int>(values) * 2);
+    };
+    // kCount pieces of a thread, `step` rows apart: the first `left` rows exist, with
+    // `valid` values from the piece on.
+    auto fetch = [&](uint32_t at, int pitch, const T *src, int64_t stride, int left, int step,
+                     int64_t valid, bool vec, auto count) {
+      constexpr int kCount = decltype(count)::value;
+      if (vec) {
+        const int bytes = clip(valid);
 #pragma unroll
-  for (int i = 0; i < kRB; ++i)
+        for (int j = 0; j < kCount; ++j) {
+          const bool in = j * step < left;
+          copy16(at + j * step * pitch, in ? src + j * step * stride : src, in ? bytes : 0);
+        }
+      } else {
+        Words w[kCount];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c[i][j] = 0.0f;
-  const T *x = static_cast<const T *>(a.x) + (g < n_rows ? rows[g] : rows[0]) * a.x_stride;
-  const int64_t kblocks = (a.H + 31) / 32;
-#pragma unroll 2
-  for (int64_t kb = unit; kb < kblocks; kb += units) {
-    const int64_t k = kb * 32 + 8 * t;
-    const uint4 q = load8(x + k, g < n_rows ? a.H - k : 0, a.vec_x);
+        for (int j = 0; j < kCount; ++j)
+          w[j] = fetch_words(src + j * step * stride, j * step < left ? valid : 0);
+#pragma unroll
+        for (int j = 0; j < kCount; ++j)
+          store16(at + j * step * pitch,
+                  join_words(w[j], src + j * step * stride, j * step < left ? valid : 0));
+      }
+    };
+    using One = std::integral_constant<int, 1>;
+    auto issue = [&](int c) {
+      if (c < chunks) {
+        const uint32_t at = ring + (c % kRowStages) * S::kStage;
+        if (c < first) {
+          const int64_t k = k0 + static_cast<int64_t>(c) * S::kK;
+          fetch(at + row1 * S::kPitchA + e1 * 2, S::kPitchA, A + row1 * a.H + k + e1, a.H,
+                a.r - row1, kStep1, k1 - k - e1, vec_a,
+                std::integral_constant<int, kR / kStep1>());
+          if (row1 < kGroup)
+            fetch(at + (kR + row1) * S::kPitchA + e1 * 2, 0, xr + k, 0, n_rows - row1, 1,
+                  k1 - k - e1, vec_x, One());
+        } else {
+          const int64_t n = n0 + static_cast<int64_t>(c - first) * S::kN;
+          fetch(at + row2 * S::kPitchB + e2 * 2, S::kPitchB, B + (n + row2) * a.r + e2, a.r,
+                static_cast<int>(n1 - n) - row2, kStep2, a.r - e2, vec_b,
+                std::integral_constant<int, S::kN / kStep2>());
+          if (rowy < kGroup)
+            fetch(at + S::kN * S::kPitchB + rowy * S::kPitchY + ey * 2, 0, yr + n, 0,
+                  n_rows - rowy, 1, n1 - n - ey, vec_y, One());
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto arrived = [&]() {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRowStages - 2) : "memory");
+      __syncthreads();
+    };
+#pragma unroll 1
+    for (int c = 0; c < kRowStages - 1; ++c) issue(c);
+    // The second product's weights come into the cache while the first one runs.
+    {
+      const char *p = reinterpret_cast<const char *>(B + n0 * a.r);
+      const int64_t bytes = (n1 - n0) * a.r * 2;
+      for (int64_t o = tid * 128; o < bytes; o += kThreads * 128)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p + o));
+    }
+
+    // v^T[rank, row]: A as the 16 rows of an instruction, x as its 8 columns.  A warp
+    // has a block of 16 ranks and every kParts-th 16 values of H.
+    const int block = warp % kRB, share = warp / kRB;
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+    for (int c = 0; c < first; ++c) {
+      arrived();
+      issue(c + kRowStages - 1);
+      const uint32_t at = ring + (c % kRowStages) * S::kStage;
+      // A stage past the end of this CTA's part holds zeros.
+#pragma unroll
+      for (int i = share; i < S::kK / 16; i += kParts) {
+        uint32_t p[4], q[2];
+        ldmatrix4(p, at + (block * 16 + (lane & 15)) * S::kPitchA + i * 32 + (lane >> 4) * 16);
+        ldmatrix2(q, at + (kR + (lane & 7)) * S::kPitchA + i * 32 + ((lane >> 3) & 1) * 16);
+        Half<T>::mma(acc, p[0], p[1], p[2], p[3], q[0], q[1]);
+      }
+    }
+    {
+      float *p = red[share] + 2 * t * kPitchV + block * 16 + g;
+      p[0] = acc[0], p[kPitchV] = acc[1];
+      p[8] = acc[2], p[kPitchV + 8] = acc[3];
+    }
+    __syncthreads();
+    for (int i = tid; i < kGroup * kPitchV; i += kThreads) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kParts; ++w) sum += red[w][i];
+      part[i] = sum;
+    }
+    const float scale = a.scale ? a.scale[s] : 1.0f;
+    cluster.sync();
+    {
+      // v, its range and its parts: a row for each warp, two neighbouring ranks a lane.
+      constexpr int kEach = (kR + 63) / 64;
+      float u[kEach][2], amax = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) u[i][0] = u[i][1] = 0.0f;
+#pragma unroll 4
+      for (int p = 0; p < C; ++p) {
+        const float *q = cluster.map_shared_rank(part, p) + warp * kPitchV + 2 * lane;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+          if (i * 64 + 2 * lane < kR) {
+            const float2 w = *reinterpret_cast<const float2 *>(q + i * 64);
+            u[i][0] += w.x, u[i][1] += w.y;
+          }
+      }
+      // The other CTAs have read this one's share when all have arrived; waited for
+      // before the next item, or at the end.
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+      float f = 1.0f;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        u[i][0] *= scale, u[i][1] *= scale;
+        amax = fmaxf(amax, fmaxf(fabsf(u[i][0]), fabsf(u[i][1])));
+      }
+      if constexpr (Half<T>::kNarrowRange)
+        f = range_factor(__uint_as_float(__reduce_max_sync(kFull, __float_as_uint(amax))));
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (i * 64 + 2 * lane < kR) {
+          uint32_t hi, lo;
+          split<T>(u[i][0] * f, u[i][1] * f, &hi, &lo);
+          *reinterpret_cast<uint32_t *>(&vhi[warp][i * 64 + 2 * lane]) = hi;
+          *reinterpret_cast<uint32_t *>(&vlo[warp][i * 64 + 2 * lane]) = lo;
+        }
+      if (lane == 0) factor[warp] = 1.0f / f;
+    }
+    __syncthreads();
+
+    // out^T[n, row]: B as the 16 rows of an instruction, v's parts as its 8 columns.
+    uint32_t hi[kRB][2], lo[kRB][2];
 #pragma unroll
     for (int i = 0; i < kRB; ++i) {
-      const int r0 = i * 16 + g, r1 = r0 + 8;
-      const uint4 u = load8(A + r0 * a.H + k, r0 < a.r ? a.H - k : 0, a.vec_a);
-      const uint4 w = load8(A + r1 * a.H + k, r1 < a.r ? a.H - k : 0, a.vec_a);
-      Half<T>::mma(c[i], u.x, w.x, u.y, w.y, q.x, q.y);
-      Half<T>::mma(c[i], u.z, w.z, u.w, w.w, q.z, q.w);
+      ldmatrix2(hi[i], smem_addr(&vhi[lane & 7][i * 16 + ((lane >> 3) & 1) * 8]));
+      ldmatrix2(lo[i], smem_addr(&vlo[lane & 7][i * 16 + ((lane >> 3) & 1) * 8]));
     }
-  }
+    const float f0 = factor[2 * t], f1 = factor[2 * t + 1];
+#pragma unroll 1
+    for (int c = first; c < chunks; ++c) {
+      arrived();
+      issue(c + kRowStages - 1);
+      unsigned char *stage = smem + (c % kRowStages) * S::kStage;
+      const uint32_t at = smem_addr(stage);
+      unsigned char *ys = stage + S::kN * S::kPitchB;
+      const int64_t n = n0 + static_cast<int64_t>(c - first) * S::kN;
+#pragma unroll 1
+      for (int b = warp * 16; b < S::kN && n + b < n1; b += kWarps * 16) {
+        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int i = 0; i < kRB; ++i) {
-    float *p = red[warp] + (i * 16 + g) * kGroup + 2 * t;
-    p[0] = c[i][0], p[1] = c[i][1];
-    p[8 * kGroup] = c[i][2], p[8 * kGroup + 1] = c[i][3];
-  }
-  __syncthreads();
-  for (int i = tid; i < kR * kGroup; i += kThreads) {
-    float sum = 0.0f;
+        for (int i = 0; i < kRB; ++i) {
+          uint32_t p[4];
+          ldmatrix4(p, at + (b + (lane & 15)) * S::kPitchB + i * 32 + (lane >> 4) * 16);
+          Half<T>::mma(d, p[0], p[1], p[2], p[3], hi[i][0], hi[i][1]);
+          Half<T>::mma(d, p[0], p[1], p[2], p[3], lo[i][0], lo[i][1]);
+        }
+        // y + update in place of y in the stage, then 16-byte pieces of out.
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) sum += red[w][i];
-    part[i] = sum;
-  }
-  cluster.sync();
-  const float scale = a.scale ? a.scale[s] : 1.0f;
-  for (int i = tid; i < kR * kGroup; i += kThreads) {
-    float sum = 0.0f;
-    for (int p = 0; p < C; ++p) sum += cluster.map_shared_rank(part, p)[i];
-    vf[i] = sum * scale;
-  }
-  // The other CTAs have read this one's share when all have arrived; waited for
-  // at the end.
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  __syncthreads();
-  {  // warp w: row w
-    float f = 1.0f;
-    if constexpr (Half<T>::kNarrowRange) {
-      float amax = 0.0f;
-      for (int i = lane; i < kR; i += 32) amax = fmaxf(amax, fabsf(vf[i * kGroup + warp]));
-      f = range_factor(__uint_as_float(__reduce_max_sync(kFull, __float_as_uint(amax))));
+        for (int j = 0; j < 4; ++j) {
+          T *p = reinterpret_cast<T *>(ys + (2 * t + (j & 1)) * S::kPitchY) + b + g + (j >> 1) * 8;
+          if (2 * t + (j & 1) < n_rows) narrow(p, widen(*p) + d[j] * (j & 1 ? f1 : f0));
+        }
+        __syncwarp();
+        const int row = lane >> 1, e = b + (lane & 1) * 8;
+        if (row < n_rows)
+          put8(static_cast<T *>(a.out) + rows[row] * a.out_stride + n + e,
+               *reinterpret_cast<const uint4 *>(ys + row * S::kPitchY + e * 2), n1 - n - e, vec_y);
+      }
     }
-    for (int i = 2 * lane; i < kR; i += 64) {
-      uint32_t hi, lo;
-      split<T>(vf[i * kGroup + warp] * f, vf[(i + 1) * kGroup + warp] * f, &hi, &lo);
-      *reinterpret_cast<uint32_t *>(&vhi[warp][i]) = hi;
-      *reinterpret_cast<uint32_t *>(&vlo[warp][i]) = lo;
-    }
-    if (kR % 32)  // the second half of the last block of 32
-      for (int i = kR + lane; i < kR + 16; i += 32) vhi[warp][i] = vlo[warp][i] = 0;
-    if (lane == 0) factor[warp] = 1.0f / f;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();  // the ring and the rows are free for the next item
   }
-  __syncthreads();
-
-  const int row0 = 2 * t, row1 = 2 * t + 1;
-  const float f0 = factor[row0], f1 = factor[row1];
-  const bool has0 = row0 < n_rows, has1 = row1 < n_rows;
-  const T *y0 = static_cast<const T *>(a.y) + (has0 ? rows[row0] : 0) * a.y_stride;
-  const T *y1 = static_cast<const T *>(a.y) + (has1 ? rows[row1] : 0) * a.y_stride;
-  T *o0 = static_cast<T *>(a.out) + (has0 ? rows[row0] : 0) * a.out_stride;
-  T *o1 = static_cast<T *>(a.out) + (has1 ? rows[row1] : 0) * a.out_stride;
-  for (int64_t nb = unit; nb < nblocks; nb += units) {
-    const int64_t n0 = nb * 16 + g, n1 = n0 + 8;
-    const bool in0 = n0 < a.N, in1 = n1 < a.N;
-    const float y00 = has0 && in0 ? widen(y0[n0]) : 0.0f, y01 = has1 && in0 ? widen(y1[n0]) : 0.0f;
-    const float y10 = has0 && in1 ? widen(y0[n1]) : 0.0f, y11 = has1 && in1 ? widen(y1[n1]) : 0.0f;
-    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int i = 0; i < (kRB + 1) / 2; ++i) {
-      const int k = i * 32 + 8 * t;
-      const uint4 u = load8(B + n0 * a.r + k, in0 ? a.r - k : 0, a.vec_b);
-      const uint4 w = load8(B + n1 * a.r + k, in1 ? a.r - k : 0, a.vec_b);
-      const uint4 h = *reinterpret_cast<const uint4 *>(&vhi[g][k]);
-      const uint4 l = *reinterpret_cast<const uint4 *>(&vlo[g][k]);
-      Half<T>::mma(d, u.x, w.x, u.y, w.y, h.x, h.y);
-      Half<T>::mma(d, u.z, w.z, u.w, w.w, h.z, h.w);
-      Half<T>::mma(d, u.x, w.x, u.y, w.y, l.x, l.y);
-      Half<T>::mma(d, u.z, w.z, u.w, w.w, l.z, l.w);
-    }
-    if (has0 && in0) narrow(o0 + n0, y00 + d[0] * f0);
-    if (has1 && in0) narrow(o1 + n0, y01 + d[1] * f1);
-    if (has0 && in1) narrow(o0 + n1, y10 + d[2] * f0);
-    if (has1 && in1) narrow(o1 + n1, y11 + d[3] * f1);
-  }
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (again) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // ---- long batches ----
@@ -480,22 +662,6 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
       if (s[j] >= 0) a.perm[at] = m0 + j * kPlanThreads + lane;
     }
   }
-}
-
-__device__ __forceinline__ uint32_t smem_addr(const void *p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-// 16 bytes into shared memory, asynchronously; bytes from `bytes` on are zeros.
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
-               : "memory");
-}
-
-__device__ __forceinline__ void store16(uint32_t dst, const uint4 &q) {
-  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(q.x), "r"(q.y), "r"(q.z),
-               "r"(q.w)
-               : "memory");
 }
 
 // mbarriers.  A wait gives up after kWaitNs or when another one of the block has:
@@ -645,9 +811,9 @@ __global__ void __launch_bounds__(kTileThreads, kVec && kRB <= 4 ? 2 : 1)
   __shared__ int failed;
 
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = cluster.num_blocks(), rank = cluster.block_rank();
+  const int log2c = a.cluster_log2, C = 1 << log2c, rank = blockIdx.x & (C - 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int tile = blockIdx.x / C;
+  const int tile = blockIdx.x >> log2c;
   if (tile >= *a.ntiles) return;
   const int4 job = a.tiles[tile];
   const int s = job.x, n_rows = job.z;
@@ -703,9 +869,10 @@ __global__ void __launch_bounds__(kTileThreads, kVec && kRB <= 4 ? 2 : 1)
   const T *A = static_cast<const T *>(a.a) + static_cast<int64_t>(s) * a.r * a.H;
   const T *B = static_cast<const T *>(a.b) + static_cast<int64_t>(s) * a.r * a.N;
   // This CTA's blocks of 64 along H and along N.
-  const int64_t kb_all = (a.H + 63) / 64, nb_all = (a.N + kNBlock - 1) / kNBlock;
-  const int k0 = static_cast<int>(kb_all * rank / C), k1 = static_cast<int>(kb_all * (rank + 1) / C);
-  const int n0 = static_cast<int>(nb_all * rank / C), n1 = static_cast<int>(nb_all * (rank + 1) / C);
+  const uint32_t kb_all = static_cast<uint32_t>((a.H + 63) / 64);
+  const uint32_t nb_all = static_cast<uint32_t>((a.N + kNBlock - 1) / kNBlock);
+  const int k0 = kb_all * rank >> log2c, k1 = kb_all * (rank + 1) >> log2c;
+  const int n0 = nb_all * rank >> log2c, n1 = nb_all * (rank + 1) >> log2c;
   const int first = k1 - k0, chunks = first + n1 - n0;
   const int k_steps = (a.r + 15) / 16;  // of the second product
 
@@ -908,14 +1075,16 @@ __global__ void __launch_bounds__(kTileThreads, kVec && kRB <= 4 ? 2 : 1)
     if (C > 1) {
       // The cluster's shares of v, added in the order of its CTAs.  They lie where v
       // will, which is written when all have read them.
-      float *share = reinterpret_cast<float *>(smem + kStages * S::kStage);
+      // Four ranks of all rows together, so that a warp reads 512 bytes in a row.
+      float4 *share = reinterpret_cast<float4 *>(smem + kStages * S::kStage) + row;
 #pragma unroll
       for (int i = 0; i < kMine; ++i)
         if (2 * i + side < kRB) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            share[((2 * i + side) * 16 + j) * kTile + row] = u[i][j];
-            u[i][j] = 0.0f;
+          for (int j = 0; j < 4; ++j) {
+            share[((2 * i + side) * 4 + j) * kTile] =
+                make_float4(u[i][4 * j], u[i][4 * j + 1], u[i][4 * j + 2], u[i][4 * j + 3]);
+            u[i][4 * j] = u[i][4 * j + 1] = u[i][4 * j + 2] = u[i][4 * j + 3] = 0.0f;
           }
         }
       asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -925,15 +1094,27 @@ __global__ void __launch_bounds__(kTileThreads, kVec && kRB <= 4 ? 2 : 1)
       }
       ok = __all_sync(kFull, ok && bar_wait<true>(shares, 0, fail));
       if (ok) {
-        for (int b = 0; b < C; ++b) {
-          const float *q = cluster.map_shared_rank(share, b) + row;
 #pragma unroll
-          for (int i = 0; i < kMine; ++i)
-            if (2 * i + side < kRB) {
+        for (int i = 0; i < kMine; ++i)
+          if (2 * i + side < kRB) {
+            for (int b = 0; b < C; b += 2) {  // C is even here
+              float4 q[2][4];
 #pragma unroll
-              for (int j = 0; j < 16; ++j) u[i][j] += q[((2 * i + side) * 16 + j) * kTile];
+              for (int h = 0; h < 2; ++h) {
+                const float4 *p =
+                    cluster.map_shared_rank(share, b + h) + (2 * i + side) * 4 * kTile;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) q[h][j] = p[j * kTile];
+              }
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  u[i][4 * j] += q[h][j].x, u[i][4 * j + 1] += q[h][j].y;
+                  u[i][4 * j + 2] += q[h][j].z, u[i][4 * j + 3] += q[h][j].w;
+                }
             }
-        }
+          }
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (ok && tid < C) bar_arrive_peer(shares_read, tid);
@@ -975,16 +1156,18 @@ __global__ void __launch_bounds__(kTileThreads, kVec && kRB <= 4 ? 2 : 1)
       tc_fence_before();
       bar_arrive(v_ready);
     }
-    for (int c = first; c < chunks && ok; ++c) {
+    // After a wait gave up, warps that meet others at a barrier still do.
+    for (int c = first; c < chunks && (ok || !vec_y); ++c) {
       const int stage = c % kStages, i = c - first, half = i & 1;
-      ok = __all_sync(kFull, bar_wait(out_done + 8 * half, (i / 2) & 1, fail) &&
+      ok = __all_sync(kFull, ok && bar_wait(out_done + 8 * half, (i / 2) & 1, fail) &&
                                  bar_wait(full + 8 * stage, (c / kStages) & 1, fail));
-      if (!ok) break;
+      if (!ok && vec_y) break;
       tc_fence_after();
       unsigned char *ys = smem + stage * S::kStage + S::kY;
       // y + update in place of y in the stage, then whole 16-byte pieces of out.
 #pragma unroll
       for (int j = 2 * side; j < 2 * side + 2; ++j) {
+        if (!ok) continue;
         float d[16];
         tc_load16(d, my_tmem + kTmemOut + half * kNBlock + j * 16);
 #pragma unroll
@@ -1001,19 +1184,54 @@ __global__ void __launch_bounds__(kTileThreads, kVec && kRB <= 4 ? 2 : 1)
         }
       }
       tc_fence_before();
-      bar_arrive(out_read + 8 * half);
-      __syncwarp();
-      const int piece = side * 4 + (lane & 3);
-      const int64_t n = static_cast<int64_t>(n0 + i) * kNBlock + piece * 8;
+      if (ok) bar_arrive(out_read + 8 * half);
+      const int64_t n = static_cast<int64_t>(n0 + i) * kNBlock;
+      if (vec_y) {
+        __syncwarp();
+        const int piece = side * 4 + (lane & 3);
 #pragma unroll
-      for (int q0 = 0; q0 < 4; ++q0) {
-        const int r = (warp & 3) * 32 + q0 * 8 + (lane >> 2);
-        if (r >= n_rows) break;
-        put8(static_cast<T *>(a.out) + rows[r] * a.out_stride + n,
-             *reinterpret_cast<const uint4 *>(ys + swizzled(r, piece)), a.N - n, vec_y);
+        for (int q0 = 0; q0 < 4; ++q0) {
+          const int r = (warp & 3) * 32 + q0 * 8 + (lane >> 2);
+          if (r >= n_rows) break;
+          put8(static_cast<T *>(a.out) + rows[r] * a.out_stride + n + piece * 8,
+               *reinterpret_cast<const uint4 *>(ys + swizzled(r, piece)), a.N - n - piece * 8,
+               true);
+        }
+      } else {
+        // Rows at any place: the aligned 16-byte words of out, nine at most, from
+        // the two pieces that each of them meets; both sides' columns together.
+        asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
+        const int word = lane & 15;
+        const int bytes = static_cast<int>(min(a.N - n, static_cast<int64_t>(kNBlock))) * 2;
+#pragma unroll 1
+        for (int q0 = 0; q0 < 8; ++q0) {
+          const int r = (warp & 3) * 32 + side * 16 + q0 * 2 + (lane >> 4);
+          if (!ok || r >= n_rows) break;
+          unsigned char *o = reinterpret_cast<unsigned char *>(static_cast<T *>(a.out) +
+                                                               rows[r] * a.out_stride + n);
+          const int off = static_cast<int>(reinterpret_cast<uintptr_t>(o) & 15);
+          const int at = word * 16 - off;  // the word's first byte in the row's columns
+          if (at >= bytes) continue;
+          const int p0 = (at + 16) / 16 - 1;  // the piece it begins in (-1: before the first)
+          Words w;
+          w.lo = *reinterpret_cast<const uint4 *>(ys + swizzled(r, max(p0, 0)));
+          w.hi = *reinterpret_cast<const uint4 *>(ys + swizzled(r, min(p0 + 1, 7)));
+          const uint4 q = join_words(w, reinterpret_cast<const T *>(static_cast<uintptr_t>(
+                                            (16 - off) & 15)), 8);
+          if (at >= 0 && at + 16 <= bytes) {
+            *reinterpret_cast<uint4 *>(o + at) = q;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (at + 2 * e >= 0 && at + 2 * e < bytes)
+                *reinterpret_cast<uint16_t *>(o + at + 2 * e) =
+                    static_cast<uint16_t>((&q.x)[e >> 1] >> (16 * (e & 1)));
+          }
+        }
+        asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
       }
       __syncwarp();
-      if (lane == 0) bar_arrive(free2 + 8 * stage);
+      if (ok && lane == 0) bar_arrive(free2 + 8 * stage);
     }
   }
   tc_fence_before();
@@ -1040,22 +1258,36 @@ int set_smem(const void *fn, int bytes) {
   return err == cudaSuccess ? XP_OK : static_cast<int>(err);
 }
 
-int launch(const void *fn, unsigned ctas, unsigned cluster, int threads, int smem,
-           const LowRankArgs &a, cudaStream_t s) {
+// `clusters` clusters of 2^log2c CTAs; where `fit` is not NULL no more than the device
+// holds at once (looked up once for a kernel and cluster size).
+int launch(const void *fn, int64_t clusters, int log2c, int threads, int smem,
+           std::atomic<int> *fit, LowRankArgs &a, cudaStream_t s) {
   int rc = set_smem(fn, smem);
   if (rc) return rc;
+  a.cluster_log2 = log2c;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas * cluster);
+  cfg.gridDim = dim3(1u << log2c);
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.x = 1u << log2c;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  void *args[] = {const_cast<LowRankArgs *>(&a)};
+  if (fit) {
+    int most = fit->load(std::memory_order_relaxed);
+    if (most == 0) {
+      cudaError_t err = cudaOccupancyMaxActiveClusters(&most, fn, &cfg);
+      if (err != cudaSuccess) return static_cast<int>(err);
+      if (most < 1) return XP_ERANGE;
+      fit->store(most, std::memory_order_relaxed);
+    }
+    if (clusters > most) clusters = most;
+  }
+  cfg.gridDim = dim3(static_cast<unsigned>(clusters) << log2c);
+  void *args[] = {&a};
   cudaError_t err = cudaLaunchKernelExC(&cfg, fn, args);
   return err == cudaSuccess ? launch_status() : static_cast<int>(err);
 }
@@ -1073,10 +1305,13 @@ int64_t scratch_need(int64_t M, int64_t slots) {
 
 template <typename T, int kRB>
 int run_sized(LowRankArgs &a, cudaStream_t s) {
+  const bool vec = a.vec_x && a.vec_a && a.vec_b && a.vec_y;
   if (a.M <= kRowsLimit) {
-    const unsigned cluster = a.M <= 16 ? 8 : 4;
-    return launch((const void *)rows_kernel<T, kRB>, static_cast<unsigned>(a.M), cluster, kThreads, 0, a,
-                  s);
+    static std::atomic<int> fit[2][2];
+    const int log2c = a.M <= 64 ? 3 : 2;
+    const void *fn = vec ? (const void *)rows_kernel<T, kRB, true>
+                         : (const void *)rows_kernel<T, kRB, false>;
+    return launch(fn, a.M, log2c, kThreads, RowsSmem<kRB>::kBytes, &fit[vec][log2c & 1], a, s);
   }
   const int bytes = 8 * (a.slots + 1);
   int rc = set_smem((const void *)plan_kernel, bytes);
@@ -1086,12 +1321,10 @@ int run_sized(LowRankArgs &a, cudaStream_t s) {
   if (rc) return rc;
   const int64_t tiles = most_tiles(a.M, a.slots);
   const int64_t full = (a.M + kTile - 1) / kTile;  // tiles of a batch with few adapters
-  const unsigned cluster = full <= 18 ? 8 : (full <= 37 ? 4 : (full <= 148 ? 2 : 1));
-  const void *fn = a.vec_x && a.vec_a && a.vec_b && a.vec_y
-                       ? (const void *)tile_kernel<T, kRB, true>
+  const int log2c = full <= 18 ? 3 : (full <= 37 ? 2 : (full <= 148 ? 1 : 0));
+  const void *fn = vec ? (const void *)tile_kernel<T, kRB, true>
                        : (const void *)tile_kernel<T, kRB, false>;
-  return launch(fn, static_cast<unsigned>(tiles), cluster, kTileThreads,
-                TileSmem<kRB>::kBytes, a, s);
+  return launch(fn, tiles, log2c, kTileThreads, TileSmem<kRB>::kBytes, nullptr, a, s);
 }
 
 template <typename T>
