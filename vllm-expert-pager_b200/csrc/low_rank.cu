@@ -136,6 +136,10 @@ __device__ __forceinline__ int slot_of_row(const LowRankArgs &a, int64_t m) {
   return s >= 0 && s < a.slots ? static_cast<int>(s) : -1;
 }
 
+__device__ __forceinline__ int place_of(const void *p) {
+  return static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
+}
+
 // Eight neighbouring values at any place, those from `valid` on as zeros (valid may
 // be <= 0): the aligned 16-byte words around them (those two that hold at least one
 // of the values), then shifts, which takes a quarter of the loads that single values
@@ -156,9 +160,8 @@ __device__ __forceinline__ Words fetch_words(const T *p, int64_t valid) {
   return w;
 }
 
-template <typename T>
-__device__ __forceinline__ uint4 join_words(const Words &v, const T *p, int64_t valid) {
-  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
+// `off`: the first value's byte in the first word.
+__device__ __forceinline__ uint4 join_words(const Words &v, int off, int64_t valid) {
   const int n = valid < 0 ? 0 : (valid < 8 ? static_cast<int>(valid) : 8);
   uint32_t w[8] = {v.lo.x, v.lo.y, v.lo.z, v.lo.w, v.hi.x, v.hi.y, v.hi.z, v.hi.w};
   if (off & 8) {
@@ -182,7 +185,7 @@ __device__ __forceinline__ uint4 join_words(const Words &v, const T *p, int64_t 
 template <typename T>
 __device__ __forceinline__ uint4 load8(const T *p, int64_t valid, bool vec) {
   if (vec && valid >= 8) return __ldg(reinterpret_cast<const uint4 *>(p));
-  return join_words(fetch_words(p, valid), p, valid);
+  return join_words(fetch_words(p, valid), place_of(p), valid);
 }
 
 // Eight neighbouring values of which `valid` exist, to any place.
@@ -411,7 +414,8 @@ __global__ void __launch_bounds__(kThreads, kVec && kRB <= 4 ? 3 : 2)
 #pragma unroll
         for (int j = 0; j < kCount; ++j)
           store16(at + j * step * pitch,
-                  join_words(w[j], src + j * step * stride, j * step < left ? valid : 0));
+                  join_words(w[j], place_of(src + j * step * stride),
+                             j * step < left ? valid : 0));
       }
     };
     using One = std::integral_constant<int, 1>;
@@ -575,17 +579,19 @@ __global__ void __launch_bounds__(kThreads, kVec && kRB <= 4 ? 3 : 2)
 // order of a slot's rows is free: a row's result does not depend on its tile.
 __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads)
     plan_kernel(const __grid_constant__ LowRankArgs a) {
-  extern __shared__ int counts[];  // [slots + 1] rows of this CTA; [slots + 1] next free place
+  // Each [slots + 1]: rows of this CTA; the next free place; rows of all CTAs.
+  extern __shared__ int counts[];
   __shared__ int sum_rows[32], sum_tiles[32];
+  // The tiles' kernel may be set up meanwhile (it waits for this one's end).
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = cluster.block_rank();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int n = a.slots + 1, M = static_cast<int>(a.M);  // the last: rows without an adapter
-  int *place = counts + n;
+  int *place = counts + n, *total = place + n;
   const int per = (M + kPlanCtas - 1) / kPlanCtas, first = min(rank * per, M),
             last = min(first + per, M);
   for (int i = tid; i < n; i += kPlanThreads) counts[i] = 0;
-  __syncthreads();
   // Four rows of a thread at a time: their ids (and map entries) come together.
   constexpr int kBatch = 4;
   auto slots_of = [&](int m0, int (&s)[kBatch]) {
@@ -599,14 +605,34 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
       }
     }
   };
-  for (int m0 = first + warp * 32; m0 < last; m0 += kBatch * kPlanThreads) {
-    int s[kBatch];
-    slots_of(m0, s);
+  auto count = [&](const int (&s)[kBatch]) {
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       const unsigned peers = __match_any_sync(kFull, s[j]);
       if (s[j] >= 0 && lane == __ffs(peers) - 1) atomicAdd(&counts[s[j]], __popc(peers));
     }
+  };
+  auto put = [&](int m0, const int (&s)[kBatch]) {
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const unsigned peers = __match_any_sync(kFull, s[j]);
+      const int leader = __ffs(peers) - 1;
+      int at = 0;
+      if (s[j] >= 0 && lane == leader) at = atomicAdd(&place[s[j]], __popc(peers));
+      at = __shfl_sync(kFull, at, leader) + __popc(peers & lanemask_lt());
+      if (s[j] >= 0) a.perm[at] = m0 + j * kPlanThreads + lane;
+    }
+  };
+  // The first batch's slots stay in registers; only longer runs are read again.
+  const int mine = first + warp * 32;
+  int s0[kBatch];
+  slots_of(mine, s0);
+  __syncthreads();
+  count(s0);
+  for (int m0 = mine + kBatch * kPlanThreads; m0 < last; m0 += kBatch * kPlanThreads) {
+    int s[kBatch];
+    slots_of(m0, s);
+    count(s);
   }
   cluster.sync();
   // Exclusive sums over the slots, a run of slots per thread; every CTA has its own.
@@ -614,16 +640,21 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
             i1 = min(i0 + run, n);
   int rows = 0, tiles = 0;
   for (int i = i0; i < i1; ++i) {
-    int all = 0, before = 0;
+    int c[kPlanCtas], all = 0, before = 0;
+#pragma unroll
+    for (int b = 0; b < kPlanCtas; ++b) c[b] = cluster.map_shared_rank(counts, b)[i];
 #pragma unroll
     for (int b = 0; b < kPlanCtas; ++b) {
       if (b == rank) before = all;
-      all += cluster.map_shared_rank(counts, b)[i];
+      all += c[b];
     }
     place[i] = before;  // of the slot's rows, those of the CTAs before this one
+    total[i] = all;
     rows += all;
     if (i < a.slots || !a.in_place) tiles += (all + kTile - 1) / kTile;
   }
+  // The counts stay until all have read them; waited for at the end.
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   int rows_before = rows, tiles_before = tiles;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -637,9 +668,7 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
   tiles_before -= tiles;
   for (int w = 0; w < warp; ++w) rows_before += sum_rows[w], tiles_before += sum_tiles[w];
   for (int i = i0; i < i1; ++i) {
-    int all = 0;
-#pragma unroll
-    for (int b = 0; b < kPlanCtas; ++b) all += cluster.map_shared_rank(counts, b)[i];
+    const int all = total[i];
     if (rank == 0 && (i < a.slots || !a.in_place))
       for (int o = 0; o < all; o += kTile)
         a.tiles[tiles_before++] =
@@ -648,20 +677,14 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     rows_before += all;
   }
   if (rank == 0 && tid == kPlanThreads - 1) *a.ntiles = tiles_before;
-  cluster.sync();  // the counts stay until all have read them
-  for (int m0 = first + warp * 32; m0 < last; m0 += kBatch * kPlanThreads) {
+  __syncthreads();
+  put(mine, s0);
+  for (int m0 = mine + kBatch * kPlanThreads; m0 < last; m0 += kBatch * kPlanThreads) {
     int s[kBatch];
     slots_of(m0, s);
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const unsigned peers = __match_any_sync(kFull, s[j]);
-      const int leader = __ffs(peers) - 1;
-      int at = 0;
-      if (s[j] >= 0 && lane == leader) at = atomicAdd(&place[s[j]], __popc(peers));
-      at = __shfl_sync(kFull, at, leader) + __popc(peers & lanemask_lt());
-      if (s[j] >= 0) a.perm[at] = m0 + j * kPlanThreads + lane;
-    }
+    put(m0, s);
   }
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // mbarriers.  A wait gives up after kWaitNs or when another one of the block has:
@@ -773,17 +796,20 @@ constexpr int kOutWarps = 8;                 // half a row of the tile for each 
 constexpr int kMmaWarp = kOutWarps;          // issues the matrix instructions
 constexpr int kLoadWarps = 4;
 constexpr int kLoaders = kLoadWarps * 32;
-constexpr int kTileThreads = (kOutWarps + 1 + kLoadWarps) * 32;
-constexpr int kStages = 3;
+constexpr int kShiftWarps = 4;               // where rows lie at any place
 constexpr int kNBlock = 64;                  // columns of out in a stage
 constexpr int kTmemCols = 256;               // v: 128 at most, then two blocks of out
 constexpr int kTmemOut = 128;
+constexpr int tile_threads(bool vec) {
+  return (kOutWarps + 1 + kLoadWarps + (vec ? 0 : kShiftWarps)) * 32;
+}
 
 // kRB: blocks of 16 ranks.  kAtoms: 128-byte rows that hold a row of ranks.
-template <int kRB>
+template <int kRB, bool kVec>
 struct TileSmem {
   static constexpr int kR = kRB * 16;
   static constexpr int kAtoms = kR > 64 ? 2 : 1;
+  static constexpr int kStages = kVec || kRB <= 4 ? 3 : 2;
   // A stage holds 128 rows x 64 values of x and kR x 64 of A, or 64 rows of B and 128 x 64 of y.
   static constexpr int kA = kTile * 128;
   static constexpr int kY = kAtoms * kNBlock * 128;
@@ -792,20 +818,28 @@ struct TileSmem {
   // The high parts of v, then the low parts; before them this CTA's share of v (32-bit).
   static constexpr int kV = 2 * kAtoms * kTile * 128;
   static_assert(kR * kTile * 4 <= kV, "a share of v has room where v goes");
-  static constexpr int kBytes = 1024 + kStages * kStage + kV;
+  // Rows at any place come as the aligned 16-byte words around them, one more than
+  // the stage's row has; shifting them fills the stage.
+  static constexpr int kWords = kVec ? 0 : (kRB <= 4 ? 4 : 2);  // such stages
+  static constexpr int kPitch = 128 + 16, kPitchB = kR * 2 + 16;
+  static constexpr int kWordsA = kTile * kPitch, kWordsY = kNBlock * kPitchB;
+  static constexpr int kWords1 = kWordsA + kR * kPitch, kWords2 = kWordsY + kTile * kPitch;
+  static constexpr int kWordsStage = kWords1 > kWords2 ? kWords1 : kWords2;
+  static constexpr int kBytes = 1024 + kStages * kStage + kV + kWords * kWordsStage;
 };
 
-// kVec: all rows allow 16-byte accesses (else each operand goes by its own flag; the
-// shifts of odd places need more registers than two CTAs on an SM leave).
+// kVec: all rows allow 16-byte accesses; else four more warps shift what the loading
+// warps bring.
 template <typename T, int kRB, bool kVec>
-__global__ void __launch_bounds__(kTileThreads, kVec && kRB <= 4 ? 2 : 1)
+__global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
     tile_kernel(const __grid_constant__ LowRankArgs a) {
-  using S = TileSmem<kRB>;
-  const bool vec_x = kVec || a.vec_x, vec_a = kVec || a.vec_a, vec_b = kVec || a.vec_b,
-             vec_y = kVec || a.vec_y;
+  using S = TileSmem<kRB, kVec>;
+  constexpr int kStages = S::kStages;
+  const bool vec_y = kVec || a.vec_y;
   extern __shared__ unsigned char raw[];
   __shared__ int64_t rows[kTile];
-  __shared__ __align__(8) uint64_t bars[3 * kStages + 8];
+  __shared__ __align__(8) uint64_t bars[3 * kStages + 8 + 2 * S::kWords];
+  __shared__ uint8_t off_x[kTile], off_y[kTile];  // rows' first bytes in their words (not kVec)
   __shared__ float amax[2][kTile];
   __shared__ uint32_t tmem_at;
   __shared__ int failed;
@@ -814,6 +848,7 @@ __global__ void __launch_bounds__(kTileThreads, kVec && kRB <= 4 ? 2 : 1)
   const int log2c = a.cluster_log2, C = 1 << log2c, rank = blockIdx.x & (C - 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int tile = blockIdx.x >> log2c;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan's end
   if (tile >= *a.ntiles) return;
   const int4 job = a.tiles[tile];
   const int s = job.x, n_rows = job.z;
@@ -822,10 +857,11 @@ __global__ void __launch_bounds__(kTileThreads, kVec && kRB <= 4 ? 2 : 1)
   const uint32_t ring = smem_addr(smem), v_at = ring + kStages * S::kStage;
   // Stage filled; stage free after the first / the second product; v in tensor
   // memory; v in shared memory; a block of out in tensor memory, and read from it;
-  // the cluster's shares of v written, and read.
+  // the cluster's shares of v written, and read; words arrived, and shifted.
   const uint32_t full = smem_addr(bars), free1 = full + 8 * kStages, free2 = free1 + 8 * kStages;
   const uint32_t v_done = free2 + 8 * kStages, v_ready = v_done + 8, out_done = v_ready + 8,
-                 out_read = out_done + 16, shares = out_read + 16, shares_read = shares + 8;
+                 out_read = out_done + 16, shares = out_read + 16, shares_read = shares + 8,
+                 words_full = shares_read + 8, words_free = words_full + 8 * S::kWords;
   volatile int *fail = &failed;
 
   if (tid < kTile) rows[tid] = a.perm[job.y + min(tid, n_rows - 1)];
@@ -833,6 +869,10 @@ __global__ void __launch_bounds__(kTileThreads, kVec && kRB <= 4 ? 2 : 1)
     __syncthreads();
     copy_rows<T>(a, n_rows, rank, C, [&](int i) { return rows[i]; });
     return;  // every CTA of the cluster
+  }
+  if (!kVec && tid < kTile) {
+    off_x[tid] = place_of(static_cast<const T *>(a.x) + rows[tid] * a.x_stride);
+    off_y[tid] = place_of(static_cast<const T *>(a.y) + rows[tid] * a.y_stride);
   }
   if (tid == 0) {
     failed = 0;
@@ -849,6 +889,10 @@ __global__ void __launch_bounds__(kTileThreads, kVec && kRB <= 4 ? 2 : 1)
     }
     bar_init(shares, C);
     bar_init(shares_read, C);
+    for (int i = 0; i < S::kWords; ++i) {
+      bar_init(words_full + 8 * i, kLoaders);
+      bar_init(words_free + 8 * i, kLoaders);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) {
@@ -878,13 +922,11 @@ __global__ void __launch_bounds__(kTileThreads, kVec && kRB <= 4 ? 2 : 1)
 
   if (warp > kMmaWarp) {
     // Loading: a thread has one 16-byte piece of every 16th row.
-    const int p = tid - (kMmaWarp + 1) * 32, piece = p & 7, row0 = p >> 3;
-    const uint32_t at0 = ring + swizzled(row0, piece);
+    const int p = (tid - (kMmaWarp + 1) * 32) % kLoaders, piece = p & 7, row0 = p >> 3;
     const int mine = (n_rows - row0 + 15) / 16;  // rows of the tile of this thread
+    const int ranks = a.r - row0;                // rows of A from this thread's first on
     constexpr int kEach = kTile / 16;
-    auto clip = [](int64_t values) {  // bytes of a piece of which `values` are left
-      return values >= 8 ? 16 : (values <= 0 ? 0 : static_cast<int>(values) * 2);
-    };
+    const int64_t k_at = static_cast<int64_t>(k0) * 64, n_at = static_cast<int64_t>(n0) * kNBlock;
     // Waits until the stage of chunk c is free; its place, 0 after a wait gave up.
     auto begin = [&](int c) {
       const int stage = c % kStages, use = c / kStages;
@@ -895,125 +937,184 @@ __global__ void __launch_bounds__(kTileThreads, kVec && kRB <= 4 ? 2 : 1)
                             : bar_wait(free2 + 8 * stage, (use - 1 - before) & 1, fail);
         if (!ok) return 0u;
       }
-      return at0 + stage * S::kStage;
+      return ring + stage * S::kStage;
     };
-    auto end = [&](int c, bool async) {
-      const uint32_t bar = full + 8 * (c % kStages);
-      if (async) {
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-      } else {
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        fence_async_proxy();
-        bar_arrive(bar);
-      }
+    auto arrive_async = [](uint32_t bar) {
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
     };
-    // Rows at any place, all of a thread's fetches under way at once.
-    auto odd_rows = [&](uint32_t at, const T *src, int64_t stride, int64_t valid) {
-      Words w[kEach];
+    if constexpr (kVec) {
+      const uint32_t at0 = swizzled(row0, piece);
+      auto clip = [](int64_t values) {  // bytes of a piece of which `values` are left
+        return values >= 8 ? 16 : (values <= 0 ? 0 : static_cast<int>(values) * 2);
+      };
+      bool ok = true;
+      {
+        const T *src[kEach];
 #pragma unroll
-      for (int j = 0; j < kEach; ++j)
-        if (j < mine) w[j] = fetch_words(src + rows[row0 + 16 * j] * stride, valid);
-#pragma unroll
-      for (int j = 0; j < kEach; ++j)
-        if (j < mine)
-          store16(at + j * 2048, join_words(w[j], src + rows[row0 + 16 * j] * stride, valid));
-    };
-    auto odd_weights = [&](uint32_t at, const T *w0, int64_t stride, int64_t left, int64_t valid,
-                           auto count) {
-      constexpr int kCount = decltype(count)::value;
-#pragma unroll
-      for (int j0 = 0; j0 < kCount; j0 += 4) {
-        Words w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (j0 + j < kCount)
-            w[j] = fetch_words(w0 + (j0 + j) * 16 * stride, 16 * (j0 + j) < left ? valid : 0);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (j0 + j < kCount)
-            store16(at + (j0 + j) * 2048, join_words(w[j], w0 + (j0 + j) * 16 * stride,
-                                                     16 * (j0 + j) < left ? valid : 0));
-      }
-    };
-
-    bool ok = true;
-    {
-      const T *src[kEach];
-#pragma unroll
-      for (int j = 0; j < kEach; ++j)
-        src[j] = static_cast<const T *>(a.x) + (j < mine ? rows[row0 + 16 * j] : 0) * a.x_stride +
-                 static_cast<int64_t>(k0) * 64 + piece * 8;
-      const T *w = A + row0 * a.H + static_cast<int64_t>(k0) * 64 + piece * 8;
-      int64_t left = a.H - static_cast<int64_t>(k0) * 64 - piece * 8;
-      const int ranks = a.r - row0;  // rows of A from this thread's first on
-      for (int c = 0; c < first; ++c, w += 64, left -= 64) {
-        const uint32_t at = begin(c);
-        if (!at) {
-          ok = false;
-          break;
-        }
-        if (vec_x) {
+        for (int j = 0; j < kEach; ++j)
+          src[j] = static_cast<const T *>(a.x) + (j < mine ? rows[row0 + 16 * j] : 0) * a.x_stride +
+                   k_at + piece * 8;
+        const T *w = A + row0 * a.H + k_at + piece * 8;
+        int64_t left = a.H - k_at - piece * 8;
+        for (int c = 0; c < first; ++c, w += 64, left -= 64) {
+          uint32_t at = begin(c);
+          if (!at) {
+            ok = false;
+            break;
+          }
+          at += at0;
           const int bytes = clip(left);
 #pragma unroll
           for (int j = 0; j < kEach; ++j) {
             if (j < mine) copy16(at + j * 2048, src[j], bytes);
             src[j] += 64;
           }
-        } else {
-          odd_rows(at, static_cast<const T *>(a.x) + static_cast<int64_t>(k0 + c) * 64 + piece * 8,
-                   a.x_stride, left);
-        }
-        if (vec_a) {
-          const int bytes = clip(left);
 #pragma unroll
           for (int j = 0; j < kRB; ++j)
             copy16(at + S::kA + j * 2048, 16 * j < ranks ? w + j * 16 * a.H : A,
                    16 * j < ranks ? bytes : 0);
-        } else {
-          odd_weights(at + S::kA, w, a.H, ranks, left, std::integral_constant<int, kRB>());
+          arrive_async(full + 8 * (c % kStages));
         }
-        end(c, vec_x && vec_a);
       }
-    }
-    if (ok) {
-      const T *src[kEach];
+      if (ok) {
+        const T *src[kEach];
 #pragma unroll
-      for (int j = 0; j < kEach; ++j)
-        src[j] = static_cast<const T *>(a.y) + (j < mine ? rows[row0 + 16 * j] : 0) * a.y_stride +
-                 static_cast<int64_t>(n0) * kNBlock + piece * 8;
-      for (int c = first; c < chunks; ++c) {
-        const uint32_t at = begin(c);
-        if (!at) break;
-        const int64_t n = static_cast<int64_t>(n0 + c - first) * kNBlock;
+        for (int j = 0; j < kEach; ++j)
+          src[j] = static_cast<const T *>(a.y) + (j < mine ? rows[row0 + 16 * j] : 0) * a.y_stride +
+                   n_at + piece * 8;
+        for (int c = first; c < chunks; ++c) {
+          uint32_t at = begin(c);
+          if (!at) break;
+          at += at0;
+          const int64_t n = static_cast<int64_t>(n0 + c - first) * kNBlock;
 #pragma unroll
-        for (int q = 0; q < S::kAtoms; ++q) {
-          const int e = q * 64 + piece * 8;
-          if (e >= S::kR) continue;
-          const T *w = B + (n + row0) * a.r + e;
-          const int64_t left = a.N - n - row0;
-          if (vec_b) {
+          for (int q = 0; q < S::kAtoms; ++q) {
+            const int e = q * 64 + piece * 8;
+            if (e >= S::kR) continue;
+            const T *w = B + (n + row0) * a.r + e;
+            const int64_t left = a.N - n - row0;
             const int bytes = clip(a.r - e);
 #pragma unroll
             for (int j = 0; j < kNBlock / 16; ++j)
               copy16(at + q * kNBlock * 128 + j * 2048, 16 * j < left ? w + j * 16 * a.r : B,
                      16 * j < left ? bytes : 0);
-          } else {
-            odd_weights(at + q * kNBlock * 128, w, a.r, left, a.r - e,
-                        std::integral_constant<int, kNBlock / 16>());
           }
-        }
-        const int64_t left = a.N - n - piece * 8;
-        if (vec_y) {
-          const int bytes = clip(left);
+          const int bytes = clip(a.N - n - piece * 8);
 #pragma unroll
           for (int j = 0; j < kEach; ++j) {
             if (j < mine) copy16(at + S::kY + j * 2048, src[j], bytes);
             src[j] += kNBlock;
           }
-        } else {
-          odd_rows(at + S::kY, static_cast<const T *>(a.y) + n + piece * 8, a.y_stride, left);
+          arrive_async(full + 8 * (c % kStages));
         }
-        end(c, vec_b && vec_y);
+      }
+    } else if (warp <= kMmaWarp + kLoadWarps) {
+      // Words: the eight of a thread's rows that begin at its piece, and the ninth of
+      // one row.  A word is read where it holds a value of the row.
+      const uint32_t words = v_at + S::kV;
+      auto begin_words = [&](int c) {
+        const int stage = c % S::kWords, use = c / S::kWords;
+        if (use > 0 && !bar_wait(words_free + 8 * stage, (use - 1) & 1, fail)) return 0u;
+        return words + stage * S::kWordsStage;
+      };
+      // `bytes`: of the row's values from the block on.
+      auto word = [](uint32_t dst, const T *row, int i, int64_t bytes) {
+        const int off = place_of(row);
+        copy16(dst, reinterpret_cast<const char *>(row) - off + i * 16,
+               i * 16 - off < bytes ? 16 : 0);
+      };
+      bool ok = true;
+      for (int c = 0; c < chunks && ok; ++c) {
+        const uint32_t at = begin_words(c);
+        ok = at != 0;
+        if (!ok) break;
+        if (c < first) {
+          const int64_t k = k_at + static_cast<int64_t>(c) * 64;
+          const int64_t bytes = min(a.H - k, static_cast<int64_t>(64)) * 2;
+          const T *x = static_cast<const T *>(a.x) + k;
+#pragma unroll
+          for (int j = 0; j < kEach; ++j)
+            if (j < mine)
+              word(at + (row0 + 16 * j) * S::kPitch + piece * 16,
+                   x + rows[row0 + 16 * j] * a.x_stride, piece, bytes);
+          if (p < n_rows) word(at + p * S::kPitch + 128, x + rows[p] * a.x_stride, 8, bytes);
+#pragma unroll
+          for (int j = 0; j < kRB; ++j)
+            if (16 * j < ranks)
+              word(at + S::kWordsA + (row0 + 16 * j) * S::kPitch + piece * 16,
+                   A + (row0 + 16 * j) * a.H + k, piece, bytes);
+          if (p < a.r) word(at + S::kWordsA + p * S::kPitch + 128, A + p * a.H + k, 8, bytes);
+        } else {
+          const int64_t n = n_at + static_cast<int64_t>(c - first) * kNBlock;
+          constexpr int kEachB = kRB * 2 + 1;  // words of a row of B
+          for (int i = p; i < kNBlock * kEachB; i += kLoaders) {
+            const int row = i / kEachB, j = i % kEachB;
+            if (n + row < a.N)
+              word(at + row * S::kPitchB + j * 16, B + (n + row) * a.r, j, a.r * 2);
+          }
+          const int64_t bytes = min(a.N - n, static_cast<int64_t>(kNBlock)) * 2;
+          const T *y = static_cast<const T *>(a.y) + n;
+#pragma unroll
+          for (int j = 0; j < kEach; ++j)
+            if (j < mine)
+              word(at + S::kWordsY + (row0 + 16 * j) * S::kPitch + piece * 16,
+                   y + rows[row0 + 16 * j] * a.y_stride, piece, bytes);
+          if (p < n_rows)
+            word(at + S::kWordsY + p * S::kPitch + 128, y + rows[p] * a.y_stride, 8, bytes);
+        }
+        arrive_async(words_full + 8 * (c % S::kWords));
+      }
+    } else {
+      // Shifting, from the words to a stage: two values a lane, a row of 64 for a warp
+      // (whole rows of shared memory, no two lanes at one bank).
+      const unsigned char *words = smem + kStages * S::kStage + S::kV;
+      const int sw = p >> 5;
+      // Values 2 i and 2 i + 1 of a row that begins `off` bytes behind src.
+      auto two = [](const unsigned char *src, int off, int i, int64_t valid) {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(src) + (off >> 2) + i;
+        uint32_t v = off & 2 ? __funnelshift_r(w[0], w[1], 16) : w[0];
+        if (2 * i + 1 >= valid) v &= 2 * i >= valid ? 0u : 0xffffu;
+        return v;
+      };
+      auto put2 = [](uint32_t at, int row, int i, uint32_t v) {
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + swizzled(row, i >> 2) + (i & 3) * 4),
+                     "r"(v)
+                     : "memory");
+      };
+      for (int c = 0; c < chunks; ++c) {
+        const int stage = c % S::kWords;
+        if (!bar_wait(words_full + 8 * stage, (c / S::kWords) & 1, fail)) break;
+        const uint32_t at = begin(c);
+        if (!at) break;
+        const unsigned char *from = words + stage * S::kWordsStage;
+        if (c < first) {
+          const int64_t k = k_at + static_cast<int64_t>(c) * 64, left = a.H - k;
+#pragma unroll 4
+          for (int row = sw; row < n_rows; row += 4)
+            put2(at, row, lane, two(from + row * S::kPitch, off_x[row], lane, left));
+#pragma unroll 4
+          for (int row = sw; row < S::kR; row += 4)
+            put2(at + S::kA, row, lane,
+                 two(from + S::kWordsA + row * S::kPitch, place_of(A + row * a.H + k), lane,
+                     row < a.r ? left : 0));
+        } else {
+          const int64_t n = n_at + static_cast<int64_t>(c - first) * kNBlock;
+          constexpr int kTwos = kRB * 8;  // of a row of B
+#pragma unroll 4
+          for (int i = p; i < kNBlock * kTwos; i += kLoaders) {
+            const int row = i / kTwos, e = i % kTwos;
+            put2(at + e / 32 * kNBlock * 128, row, e % 32,
+                 two(from + row * S::kPitchB, place_of(B + (n + row) * a.r), e,
+                     n + row < a.N ? a.r : 0));
+          }
+#pragma unroll 4
+          for (int row = sw; row < n_rows; row += 4)
+            put2(at + S::kY, row, lane,
+                 two(from + S::kWordsY + row * S::kPitch, off_y[row], lane, a.N - n));
+        }
+        fence_async_proxy();
+        bar_arrive(full + 8 * (c % kStages));
+        bar_arrive(words_free + 8 * stage);
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -1102,7 +1203,8 @@ __global__ void __launch_bounds__(kTileThreads, kVec && kRB <= 4 ? 2 : 1)
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 const float4 *p =
-                    cluster.map_shared_rank(share, b + h) + (2 * i + side) * 4 * kTile;
+                    (b + h == rank ? share : cluster.map_shared_rank(share, b + h)) +
+                    (2 * i + side) * 4 * kTile;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) q[h][j] = p[j * kTile];
               }
@@ -1198,35 +1300,25 @@ __global__ void __launch_bounds__(kTileThreads, kVec && kRB <= 4 ? 2 : 1)
                true);
         }
       } else {
-        // Rows at any place: the aligned 16-byte words of out, nine at most, from
-        // the two pieces that each of them meets; both sides' columns together.
+        // Rows at any place: a row of the block for a warp, the aligned pairs of its
+        // values (the first or last value alone); both sides' columns together.
         asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
-        const int word = lane & 15;
-        const int bytes = static_cast<int>(min(a.N - n, static_cast<int64_t>(kNBlock))) * 2;
-#pragma unroll 1
-        for (int q0 = 0; q0 < 8; ++q0) {
-          const int r = (warp & 3) * 32 + side * 16 + q0 * 2 + (lane >> 4);
-          if (!ok || r >= n_rows) break;
-          unsigned char *o = reinterpret_cast<unsigned char *>(static_cast<T *>(a.out) +
-                                                               rows[r] * a.out_stride + n);
-          const int off = static_cast<int>(reinterpret_cast<uintptr_t>(o) & 15);
-          const int at = word * 16 - off;  // the word's first byte in the row's columns
-          if (at >= bytes) continue;
-          const int p0 = (at + 16) / 16 - 1;  // the piece it begins in (-1: before the first)
-          Words w;
-          w.lo = *reinterpret_cast<const uint4 *>(ys + swizzled(r, max(p0, 0)));
-          w.hi = *reinterpret_cast<const uint4 *>(ys + swizzled(r, min(p0 + 1, 7)));
-          const uint4 q = join_words(w, reinterpret_cast<const T *>(static_cast<uintptr_t>(
-                                            (16 - off) & 15)), 8);
-          if (at >= 0 && at + 16 <= bytes) {
-            *reinterpret_cast<uint4 *>(o + at) = q;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (at + 2 * e >= 0 && at + 2 * e < bytes)
-                *reinterpret_cast<uint16_t *>(o + at + 2 * e) =
-                    static_cast<uint16_t>((&q.x)[e >> 1] >> (16 * (e & 1)));
-          }
+        const int left = static_cast<int>(min(a.N - n, static_cast<int64_t>(kNBlock)));
+        auto value = [&](int r, int e) {
+          return *reinterpret_cast<const uint16_t *>(ys + swizzled(r, e >> 3) + (e & 7) * 2);
+        };
+        const int r0 = (warp & 3) * 32 + side * 16;
+#pragma unroll 4
+        for (int r = r0; r < min(r0 + 16, n_rows); ++r) {
+          if (!ok) break;
+          uint16_t *o = static_cast<uint16_t *>(a.out) + rows[r] * a.out_stride + n;
+          const int e = 2 * lane + (place_of(o) >> 1 & 1);
+          if (e + 1 < left)
+            *reinterpret_cast<uint32_t *>(o + e) =
+                value(r, e) | static_cast<uint32_t>(value(r, e + 1)) << 16;
+          else if (e < left)
+            o[e] = value(r, e);
+          if (lane == 0 && e == 1) o[0] = value(r, 0);
         }
         asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
       }
@@ -1247,7 +1339,7 @@ __global__ void __launch_bounds__(kTileThreads, kVec && kRB <= 4 ? 2 : 1)
   if (failed) {  // a wait gave up: the rows must not pass for results
     for (int i = 0; i < n_rows; ++i)
       for (int64_t n = static_cast<int64_t>(n0) * kNBlock + tid;
-           n < min(a.N, static_cast<int64_t>(n1) * kNBlock); n += kTileThreads)
+           n < min(a.N, static_cast<int64_t>(n1) * kNBlock); n += blockDim.x)
         narrow(static_cast<T *>(a.out) + rows[i] * a.out_stride + n, NAN);
   }
 }
@@ -1259,9 +1351,10 @@ int set_smem(const void *fn, int bytes) {
 }
 
 // `clusters` clusters of 2^log2c CTAs; where `fit` is not NULL no more than the device
-// holds at once (looked up once for a kernel and cluster size).
+// holds at once (looked up once for a kernel and cluster size).  `early`: the launch
+// may begin before the kernel before it has ended (it waits for that end itself).
 int launch(const void *fn, int64_t clusters, int log2c, int threads, int smem,
-           std::atomic<int> *fit, LowRankArgs &a, cudaStream_t s) {
+           std::atomic<int> *fit, bool early, LowRankArgs &a, cudaStream_t s) {
   int rc = set_smem(fn, smem);
   if (rc) return rc;
   a.cluster_log2 = log2c;
@@ -1270,12 +1363,14 @@ int launch(const void *fn, int64_t clusters, int log2c, int threads, int smem,
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 1u << log2c;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = early ? 2 : 1;
   if (fit) {
     int most = fit->load(std::memory_order_relaxed);
     if (most == 0) {
@@ -1311,9 +1406,10 @@ int run_sized(LowRankArgs &a, cudaStream_t s) {
     const int log2c = a.M <= 64 ? 3 : 2;
     const void *fn = vec ? (const void *)rows_kernel<T, kRB, true>
                          : (const void *)rows_kernel<T, kRB, false>;
-    return launch(fn, a.M, log2c, kThreads, RowsSmem<kRB>::kBytes, &fit[vec][log2c & 1], a, s);
+    return launch(fn, a.M, log2c, kThreads, RowsSmem<kRB>::kBytes, &fit[vec][log2c & 1], false, a,
+                  s);
   }
-  const int bytes = 8 * (a.slots + 1);
+  const int bytes = 12 * (a.slots + 1);
   int rc = set_smem((const void *)plan_kernel, bytes);
   if (rc) return rc;
   plan_kernel<<<kPlanCtas, kPlanThreads, bytes, s>>>(a);
@@ -1324,7 +1420,8 @@ int run_sized(LowRankArgs &a, cudaStream_t s) {
   const int log2c = full <= 18 ? 3 : (full <= 37 ? 2 : (full <= 148 ? 1 : 0));
   const void *fn = vec ? (const void *)tile_kernel<T, kRB, true>
                        : (const void *)tile_kernel<T, kRB, false>;
-  return launch(fn, tiles, log2c, kTileThreads, TileSmem<kRB>::kBytes, nullptr, a, s);
+  const int smem = vec ? TileSmem<kRB, true>::kBytes : TileSmem<kRB, false>::kBytes;
+  return launch(fn, tiles, log2c, tile_threads(vec), smem, nullptr, true, a, s);
 }
 
 template <typename T>
