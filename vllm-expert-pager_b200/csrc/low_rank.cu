@@ -839,7 +839,11 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
   extern __shared__ unsigned char raw[];
   __shared__ int64_t rows[kTile];
   __shared__ __align__(8) uint64_t bars[3 * kStages + 8 + 2 * S::kWords];
-  __shared__ uint8_t off_x[kTile], off_y[kTile];  // rows' first bytes in their words (not kVec)
+  // Not kVec: where a row's first value lies in its words (bytes), and in the upper
+  // half the bits to shift by; the rows' first values of out in this CTA's part.
+  __shared__ uint32_t at_x[kVec ? 1 : kTile], at_y[kVec ? 1 : kTile], at_a[kVec ? 1 : S::kR],
+      at_b[kVec ? 1 : kNBlock];
+  __shared__ uint16_t *out_row[kVec ? 1 : kTile];
   __shared__ float amax[2][kTile];
   __shared__ uint32_t tmem_at;
   __shared__ int failed;
@@ -869,10 +873,6 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
     __syncthreads();
     copy_rows<T>(a, n_rows, rank, C, [&](int i) { return rows[i]; });
     return;  // every CTA of the cluster
-  }
-  if (!kVec && tid < kTile) {
-    off_x[tid] = place_of(static_cast<const T *>(a.x) + rows[tid] * a.x_stride);
-    off_y[tid] = place_of(static_cast<const T *>(a.y) + rows[tid] * a.y_stride);
   }
   if (tid == 0) {
     failed = 0;
@@ -919,6 +919,22 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
   const int n0 = nb_all * rank >> log2c, n1 = nb_all * (rank + 1) >> log2c;
   const int first = k1 - k0, chunks = first + n1 - n0;
   const int k_steps = (a.r + 15) / 16;  // of the second product
+  if constexpr (!kVec) {
+    // Blocks are whole words apart, so these hold for every block.
+    auto place = [](const T *row, int pitch, int i) {
+      const int off = place_of(row);
+      return static_cast<uint32_t>(i * pitch + (off & 12)) | (off & 2 ? 16u << 16 : 0u);
+    };
+    if (tid < kTile) {
+      at_x[tid] = place(static_cast<const T *>(a.x) + rows[tid] * a.x_stride, S::kPitch, tid);
+      at_y[tid] = place(static_cast<const T *>(a.y) + rows[tid] * a.y_stride, S::kPitch, tid);
+      out_row[tid] = static_cast<uint16_t *>(a.out) + rows[tid] * a.out_stride +
+                     static_cast<int64_t>(n0) * kNBlock;
+    }
+    if (tid < S::kR) at_a[tid] = place(A + tid * a.H, S::kPitch, tid);
+    if (tid < kNBlock) at_b[tid] = place(B + tid * a.r, S::kPitchB, tid);
+    __syncthreads();
+  }
 
   if (warp > kMmaWarp) {
     // Loading: a thread has one 16-byte piece of every 16th row.
@@ -1023,45 +1039,64 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
         copy16(dst, reinterpret_cast<const char *>(row) - off + i * 16,
                i * 16 - off < bytes ? 16 : 0);
       };
+      // The words of up to eight rows of x or y: kept as addresses, and the rows'
+      // places in their first words (four bits each).
+      const char *src[kEach], *ninth;
+      uint32_t offs = 0;
+      int off9 = 0;
+      auto aim = [&](const T *base, int64_t stride) {
+        offs = 0;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+          const T *row = base + (j < mine ? rows[row0 + 16 * j] : 0) * stride;
+          offs |= static_cast<uint32_t>(place_of(row)) << (4 * j);
+          src[j] = reinterpret_cast<const char *>(row) - place_of(row) + piece * 16;
+        }
+        const T *row = base + (p < n_rows ? rows[p] : 0) * stride;
+        off9 = place_of(row);
+        ninth = reinterpret_cast<const char *>(row) - off9 + 128;
+      };
+      auto fetch = [&](uint32_t at, int bytes) {
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+          if (j < mine)
+            copy16(at + (row0 + 16 * j) * S::kPitch + piece * 16, src[j],
+                   piece * 16 - static_cast<int>(offs >> (4 * j) & 15) < bytes ? 16 : 0);
+          src[j] += 128;
+        }
+        if (p < n_rows) copy16(at + p * S::kPitch + 128, ninth, 128 - off9 < bytes ? 16 : 0);
+        ninth += 128;
+      };
       bool ok = true;
-      for (int c = 0; c < chunks && ok; ++c) {
+      aim(static_cast<const T *>(a.x) + k_at, a.x_stride);
+      for (int c = 0; c < first; ++c) {
         const uint32_t at = begin_words(c);
         ok = at != 0;
         if (!ok) break;
-        if (c < first) {
-          const int64_t k = k_at + static_cast<int64_t>(c) * 64;
-          const int64_t bytes = min(a.H - k, static_cast<int64_t>(64)) * 2;
-          const T *x = static_cast<const T *>(a.x) + k;
+        const int64_t k = k_at + static_cast<int64_t>(c) * 64;
+        const int bytes = static_cast<int>(min(a.H - k, static_cast<int64_t>(64))) * 2;
+        fetch(at, bytes);
 #pragma unroll
-          for (int j = 0; j < kEach; ++j)
-            if (j < mine)
-              word(at + (row0 + 16 * j) * S::kPitch + piece * 16,
-                   x + rows[row0 + 16 * j] * a.x_stride, piece, bytes);
-          if (p < n_rows) word(at + p * S::kPitch + 128, x + rows[p] * a.x_stride, 8, bytes);
-#pragma unroll
-          for (int j = 0; j < kRB; ++j)
-            if (16 * j < ranks)
-              word(at + S::kWordsA + (row0 + 16 * j) * S::kPitch + piece * 16,
-                   A + (row0 + 16 * j) * a.H + k, piece, bytes);
-          if (p < a.r) word(at + S::kWordsA + p * S::kPitch + 128, A + p * a.H + k, 8, bytes);
-        } else {
-          const int64_t n = n_at + static_cast<int64_t>(c - first) * kNBlock;
-          constexpr int kEachB = kRB * 2 + 1;  // words of a row of B
-          for (int i = p; i < kNBlock * kEachB; i += kLoaders) {
-            const int row = i / kEachB, j = i % kEachB;
-            if (n + row < a.N)
-              word(at + row * S::kPitchB + j * 16, B + (n + row) * a.r, j, a.r * 2);
-          }
-          const int64_t bytes = min(a.N - n, static_cast<int64_t>(kNBlock)) * 2;
-          const T *y = static_cast<const T *>(a.y) + n;
-#pragma unroll
-          for (int j = 0; j < kEach; ++j)
-            if (j < mine)
-              word(at + S::kWordsY + (row0 + 16 * j) * S::kPitch + piece * 16,
-                   y + rows[row0 + 16 * j] * a.y_stride, piece, bytes);
-          if (p < n_rows)
-            word(at + S::kWordsY + p * S::kPitch + 128, y + rows[p] * a.y_stride, 8, bytes);
+        for (int j = 0; j < kRB; ++j)
+          if (16 * j < ranks)
+            word(at + S::kWordsA + (row0 + 16 * j) * S::kPitch + piece * 16,
+                 A + (row0 + 16 * j) * a.H + k, piece, bytes);
+        if (p < a.r) word(at + S::kWordsA + p * S::kPitch + 128, A + p * a.H + k, 8, bytes);
+        arrive_async(words_full + 8 * (c % S::kWords));
+      }
+      aim(static_cast<const T *>(a.y) + n_at, a.y_stride);
+      for (int c = first; c < chunks && ok; ++c) {
+        const uint32_t at = begin_words(c);
+        if (!at) break;
+        const int64_t n = n_at + static_cast<int64_t>(c - first) * kNBlock;
+        constexpr int kEachB = kRB * 2 + 1;  // words of a row of B
+        for (int i = p; i < kNBlock * kEachB; i += kLoaders) {
+          const int row = i / kEachB, j = i % kEachB;
+          if (n + row < a.N)
+            word(at + row * S::kPitchB + j * 16, B + (n + row) * a.r, j, a.r * 2);
         }
+        fetch(at + S::kWordsY,
+              static_cast<int>(min(a.N - n, static_cast<int64_t>(kNBlock))) * 2);
         arrive_async(words_full + 8 * (c % S::kWords));
       }
     } else {
@@ -1069,17 +1104,32 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
       // (whole rows of shared memory, no two lanes at one bank).
       const unsigned char *words = smem + kStages * S::kStage + S::kV;
       const int sw = p >> 5;
-      // Values 2 i and 2 i + 1 of a row that begins `off` bytes behind src.
-      auto two = [](const unsigned char *src, int off, int i, int64_t valid) {
-        const uint32_t *w = reinterpret_cast<const uint32_t *>(src) + (off >> 2) + i;
-        uint32_t v = off & 2 ? __funnelshift_r(w[0], w[1], 16) : w[0];
-        if (2 * i + 1 >= valid) v &= 2 * i >= valid ? 0u : 0xffffu;
-        return v;
+      // Values 2 i and 2 i + 1 of the row at `place` (see above).
+      auto two = [](const unsigned char *src, uint32_t place, int i) {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(src + (place & 0xffff)) + i;
+        return __funnelshift_r(w[0], w[1], place >> 16);
       };
-      auto put2 = [](uint32_t at, int row, int i, uint32_t v) {
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + swizzled(row, i >> 2) + (i & 3) * 4),
-                     "r"(v)
-                     : "memory");
+      // Of two values those of which `valid` from the first on exist.
+      auto keep = [](int64_t valid) { return valid >= 2 ? ~0u : (valid == 1 ? 0xffffu : 0u); };
+      auto put2 = [](uint32_t at, uint32_t v) {
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+      };
+      // A lane's place in rows of this warp (row % 8 is sw or sw + 4).
+      const uint32_t lane_at[2] = {
+          static_cast<uint32_t>(swizzled(sw, lane >> 2) + (lane & 3) * 4),
+          static_cast<uint32_t>(swizzled(sw + 4, lane >> 2) + (lane & 3) * 4 - 512)};
+      // Rows sw, sw + 4, ... of x or y, eight at a time (the last eight may run past
+      // n_rows: rows of the stage that nothing reads).
+      auto shift_rows = [&](uint32_t at, const unsigned char *src, const uint32_t *place,
+                            int count, uint32_t mask) {
+#pragma unroll 1
+        for (int j0 = 0; 4 * j0 < count; j0 += 8) {
+          uint32_t v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = two(src, place[sw + 4 * (j0 + j)], lane) & mask;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) put2(at + lane_at[j & 1] + (j0 + j) * 512, v[j]);
+        }
       };
       for (int c = 0; c < chunks; ++c) {
         const int stage = c % S::kWords;
@@ -1088,29 +1138,37 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
         if (!at) break;
         const unsigned char *from = words + stage * S::kWordsStage;
         if (c < first) {
-          const int64_t k = k_at + static_cast<int64_t>(c) * 64, left = a.H - k;
-#pragma unroll 4
-          for (int row = sw; row < n_rows; row += 4)
-            put2(at, row, lane, two(from + row * S::kPitch, off_x[row], lane, left));
-#pragma unroll 4
-          for (int row = sw; row < S::kR; row += 4)
-            put2(at + S::kA, row, lane,
-                 two(from + S::kWordsA + row * S::kPitch, place_of(A + row * a.H + k), lane,
-                     row < a.r ? left : 0));
+          const uint32_t mask = keep(a.H - k_at - static_cast<int64_t>(c) * 64 - 2 * lane);
+          shift_rows(at, from, at_x, n_rows, mask);
+#pragma unroll
+          for (int j0 = 0; j0 < S::kR / 4; j0 += 4) {
+            uint32_t v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int row = sw + 4 * (j0 + j);
+              v[j] = row < a.r ? two(from + S::kWordsA, at_a[row], lane) & mask : 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) put2(at + S::kA + lane_at[j & 1] + (j0 + j) * 512, v[j]);
+          }
         } else {
           const int64_t n = n_at + static_cast<int64_t>(c - first) * kNBlock;
           constexpr int kTwos = kRB * 8;  // of a row of B
-#pragma unroll 4
-          for (int i = p; i < kNBlock * kTwos; i += kLoaders) {
-            const int row = i / kTwos, e = i % kTwos;
-            put2(at + e / 32 * kNBlock * 128, row, e % 32,
-                 two(from + row * S::kPitchB, place_of(B + (n + row) * a.r), e,
-                     n + row < a.N ? a.r : 0));
+#pragma unroll 1
+          for (int i0 = p; i0 < kNBlock * kTwos; i0 += 4 * kLoaders) {
+            uint32_t v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int row = (i0 + j * kLoaders) / kTwos, e = (i0 + j * kLoaders) % kTwos;
+              v[j] = n + row < a.N ? two(from, at_b[row], e) & keep(a.r - 2 * e) : 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int row = (i0 + j * kLoaders) / kTwos, e = (i0 + j * kLoaders) % kTwos;
+              put2(at + e / 32 * kNBlock * 128 + swizzled(row, e % 32 >> 2) + (e & 3) * 4, v[j]);
+            }
           }
-#pragma unroll 4
-          for (int row = sw; row < n_rows; row += 4)
-            put2(at + S::kY, row, lane,
-                 two(from + S::kWordsY + row * S::kPitch, off_y[row], lane, a.N - n));
+          shift_rows(at + S::kY, from + S::kWordsY, at_y, n_rows, keep(a.N - n - 2 * lane));
         }
         fence_async_proxy();
         bar_arrive(full + 8 * (c % kStages));
@@ -1270,19 +1328,21 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
 #pragma unroll
       for (int j = 2 * side; j < 2 * side + 2; ++j) {
         if (!ok) continue;
+        uint4 q[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          q[h] = *reinterpret_cast<const uint4 *>(ys + swizzled(row, 2 * j + h));
         float d[16];
         tc_load16(d, my_tmem + kTmemOut + half * kNBlock + j * 16);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint4 *p = reinterpret_cast<uint4 *>(ys + swizzled(row, 2 * j + h));
-          uint4 q = *p;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 w = Half<T>::unpack((&q.x)[e]);
-            (&q.x)[e] = Half<T>::pack(w.x + d[h * 8 + 2 * e] * back,
-                                      w.y + d[h * 8 + 2 * e + 1] * back);
+            const float2 w = Half<T>::unpack((&q[h].x)[e]);
+            (&q[h].x)[e] = Half<T>::pack(w.x + d[h * 8 + 2 * e] * back,
+                                         w.y + d[h * 8 + 2 * e + 1] * back);
           }
-          *p = q;
+          *reinterpret_cast<uint4 *>(ys + swizzled(row, 2 * j + h)) = q[h];
         }
       }
       tc_fence_before();
@@ -1291,34 +1351,51 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
       if (vec_y) {
         __syncwarp();
         const int piece = side * 4 + (lane & 3);
+        uint4 q[4];
 #pragma unroll
-        for (int q0 = 0; q0 < 4; ++q0) {
-          const int r = (warp & 3) * 32 + q0 * 8 + (lane >> 2);
-          if (r >= n_rows) break;
-          put8(static_cast<T *>(a.out) + rows[r] * a.out_stride + n + piece * 8,
-               *reinterpret_cast<const uint4 *>(ys + swizzled(r, piece)), a.N - n - piece * 8,
-               true);
+        for (int j = 0; j < 4; ++j)
+          q[j] = *reinterpret_cast<const uint4 *>(
+              ys + swizzled((warp & 3) * 32 + j * 8 + (lane >> 2), piece));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = (warp & 3) * 32 + j * 8 + (lane >> 2);
+          if (r < n_rows)
+            put8(static_cast<T *>(a.out) + rows[r] * a.out_stride + n + piece * 8, q[j],
+                 a.N - n - piece * 8, true);
         }
       } else {
         // Rows at any place: a row of the block for a warp, the aligned pairs of its
         // values (the first or last value alone); both sides' columns together.
         asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
         const int left = static_cast<int>(min(a.N - n, static_cast<int64_t>(kNBlock)));
-        auto value = [&](int r, int e) {
-          return *reinterpret_cast<const uint16_t *>(ys + swizzled(r, e >> 3) + (e & 7) * 2);
-        };
         const int r0 = (warp & 3) * 32 + side * 16;
-#pragma unroll 4
-        for (int r = r0; r < min(r0 + 16, n_rows); ++r) {
-          if (!ok) break;
-          uint16_t *o = static_cast<uint16_t *>(a.out) + rows[r] * a.out_stride + n;
-          const int e = 2 * lane + (place_of(o) >> 1 & 1);
-          if (e + 1 < left)
-            *reinterpret_cast<uint32_t *>(o + e) =
-                value(r, e) | static_cast<uint32_t>(value(r, e + 1)) << 16;
-          else if (e < left)
-            o[e] = value(r, e);
-          if (lane == 0 && e == 1) o[0] = value(r, 0);
+        const uint32_t here = (lane >> 2) * 16 + (lane & 3) * 4,
+                       next = (lane + 1 >> 2) * 16 + (lane + 1 & 3) * 4;
+#pragma unroll 1
+        for (int j0 = 0; j0 < 16 && ok && r0 + j0 < n_rows; j0 += 8) {
+          uint16_t *o[8];
+          uint32_t v[8], v0[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int r = r0 + j0 + j;
+            const unsigned char *row = ys + r * 128;
+            const uint32_t turn = (r & 7) << 4;
+            o[j] = out_row[r] + static_cast<int64_t>(i) * kNBlock;
+            v0[j] = *reinterpret_cast<const uint32_t *>(row + (here ^ turn));
+            v[j] = __funnelshift_r(
+                v0[j], *reinterpret_cast<const uint32_t *>(row + ((next & 127) ^ turn)),
+                (place_of(o[j]) & 2) * 8);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (r0 + j0 + j >= n_rows) break;
+            const int odd = place_of(o[j]) >> 1 & 1, pairs = (left - odd) >> 1;
+            if (lane < pairs)
+              *reinterpret_cast<uint32_t *>(o[j] + odd + 2 * lane) = v[j];
+            else if (lane == pairs && (left - odd & 1))
+              o[j][odd + 2 * lane] = static_cast<uint16_t>(v[j]);
+            if (lane == 0 && odd) o[j][0] = static_cast<uint16_t>(v0[j]);
+          }
         }
         asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
       }
