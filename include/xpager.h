@@ -348,8 +348,8 @@ int xp_route_backward(const void *logits, int dtype, int64_t T, int64_t E, int64
  *
  * No counterpart in the reference.  out[m] = y[m] + scale[s] * (x[m] A_s^T) B_s^T
  * for every row m < M, where s is the slot of the row's adapter: ids[m], or
- * slot_of[ids[m]] when slot_of (int32[adapters], an expert_map of
- * xp_acquire_pair) is not NULL.  A row whose id or slot is out of range has no
+ * slot_of[ids[m]] when slot_of ([adapters] of slot_bytes 4 or 8: an expert_map of
+ * xp_acquire_pair, or a table's slot_of) is not NULL.  A row whose id or slot is out of range has no
  * adapter: out[m] = y[m].  x: M rows of H values, y and out: M rows of N values,
  * a: [slots][r][H], b: [slots][N][r] (both contiguous), all of type dtype
  * (XP_BF16 or XP_F16); the strides count elements from row to row.  scale:
@@ -364,8 +364,8 @@ int64_t xp_low_rank_scratch_bytes(int64_t M, int64_t slots);
 int xp_add_low_rank(const void *x, int64_t x_stride, const void *y, int64_t y_stride, void *out,
                     int64_t out_stride, int dtype, int64_t M, int64_t H, int64_t N, int64_t r,
                     const void *a, const void *b, int64_t slots, const float *scale,
-                    const void *ids, int ids_bytes, const int32_t *slot_of, int64_t adapters,
-                    void *scratch, int64_t scratch_bytes, void *stream);
+                    const void *ids, int ids_bytes, const void *slot_of, int slot_bytes,
+                    int64_t adapters, void *scratch, int64_t scratch_bytes, void *stream);
 
 /* ---- host side ---- */
 

@@ -154,6 +154,9 @@ def test_slot_map(M):
     slots[slots >= S] = -1
     for t in (torch.int32, torch.int64):
         check(o, ids.to(t), slots, slot_map=slot_map, out=fresh(o))
+    wide = slot_map.long()
+    wide[62] = -(1 << 40)
+    check(o, ids.to(torch.int32), slots, slot_map=wide, out=fresh(o))
     check(o, slots.to(torch.int32), slots, scale=None, out=fresh(o))
 
 
@@ -292,3 +295,136 @@ def test_replays_in_graphs_and_on_streams(M):
             outs.append(step())
     torch.cuda.synchronize()
     assert all(torch.equal(out, want) for out in outs)
+
+
+# ---- the pager ----
+
+def adapter(num, r, H, N, dtype, g):
+    a = (torch.randn((r, H), generator=g) / math.sqrt(H)).to(dtype)
+    b = (torch.randn((N, r), generator=g) / math.sqrt(r)).to(dtype)
+    return a, b, 0.5 + float(torch.rand((), generator=g))
+
+
+def pager_of(num, slots, rank, H, N, dtype, seed=0):
+    from vllm_expert_pager.adapters import AdapterPager
+
+    g = torch.Generator().manual_seed(seed)
+    pager = AdapterPager(num, slots, rank, H, N, dtype, DEV)
+    all_ = [adapter(i, 1 + i % rank, H, N, dtype, g) for i in range(num)]
+    for i, (a, b, f) in enumerate(all_):
+        pager.write(i, a, b, f)
+    return pager, all_, g
+
+
+def slabs(all_, rank, H, N, dtype):
+    """All adapters as slabs padded to one rank."""
+    a = torch.zeros((len(all_), rank, H), dtype=dtype, device=DEV)
+    b = torch.zeros((len(all_), N, rank), dtype=dtype, device=DEV)
+    for i, (u, w, _) in enumerate(all_):
+        a[i, : u.shape[0]] = u.to(DEV)
+        b[i, :, : u.shape[0]] = w.to(DEV)
+    return a, b, torch.tensor([f for *_, f in all_], device=DEV)
+
+
+@pytest.mark.parametrize("rank, H, N", [(12, 96, 72), (16, 257, 131)])
+def test_pager_serves_more_adapters_than_slots(rank, H, N):
+    num, S, dtype = 40, 6, torch.bfloat16
+    pager, all_, g = pager_of(num, S, rank, H, N, dtype)
+    try:
+        for step in range(30):
+            M = (1, 9, 700)[step % 3]
+            requests = torch.randint(-1, num, (S,), generator=g)
+            ids = requests[torch.randint(0, S, (M,), generator=g)]
+            y = torch.randn((M, N), generator=g).to(dtype).to(DEV)
+            x = torch.randn((M, H), generator=g).to(dtype).to(DEV)
+            if step == 11:  # an adapter that is in a slot gets new weights
+                i = int(requests.clamp(min=0)[0])
+                all_[i] = adapter(i, rank, H, N, dtype, g)
+                pager.write(i, *all_[i])
+            slot = pager.page(requests.to(DEV))
+            got = pager.add(y, x, ids.to(DEV), out=torch.empty_like(y))
+            a, b, f = slabs(all_, rank, H, N, dtype)
+            want, bound = reference(y, x, a, b, ids.to(DEV), f)
+            assert ((got.double() - want).abs() <= bound).all(), step
+            live = requests[requests >= 0].unique()
+            assert (slot[live.to(DEV)] >= 0).all()
+            assert int((slot >= 0).sum()) <= S
+        assert int(pager.table.misses) > S and int(pager.table.hits) > 0
+        with pytest.raises(ValueError, match="at most 6 adapters"):
+            pager.page(torch.zeros((7,), dtype=torch.int32, device=DEV))
+        # A row whose adapter is in host memory only keeps y.
+        out_of = int((pager.slot_map < 0).nonzero()[0])
+        got = pager.add(y, x, torch.full((M,), out_of, device=DEV), out=torch.empty_like(y))
+        assert torch.equal(got, y)
+    finally:
+        pager.release()
+    with pytest.raises(RuntimeError, match="released"):
+        pager.page(torch.zeros((1,), dtype=torch.int32, device=DEV))
+
+
+def test_pager_step_replays_in_a_graph():
+    num, S, rank, H, N, M, dtype = 24, 5, 8, 128, 64, 33, torch.float16
+    pager, all_, g = pager_of(num, S, rank, H, N, dtype, seed=3)
+    try:
+        requests = torch.zeros((S,), dtype=torch.int32, device=DEV)
+        rows = torch.zeros((M,), dtype=torch.int64, device=DEV)
+        x = torch.zeros((M, H), dtype=dtype, device=DEV)
+        y = torch.zeros((M, N), dtype=dtype, device=DEV)
+        out = torch.empty_like(y)
+        pager.page(requests)
+        pager.add(y, x, rows, out=out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            pager.page(requests)
+            pager.add(y, x, rows, out=out)
+            with pytest.raises(RuntimeError, match="during a capture"):
+                pager.write(0, *all_[0])
+        a, b, f = slabs(all_, rank, H, N, dtype)
+        for _ in range(12):
+            new = torch.randint(-1, num, (S,), generator=g)
+            ids = new[torch.randint(0, S, (M,), generator=g)]
+            requests.copy_(new)
+            rows.copy_(ids)
+            x.copy_(torch.randn((M, H), generator=g))
+            y.copy_(torch.randn((M, N), generator=g))
+            graph.replay()
+            torch.cuda.synchronize()
+            want, bound = reference(y, x, a, b, ids.to(DEV), f)
+            assert ((out.double() - want).abs() <= bound).all()
+        del graph
+    finally:
+        pager.release()
+
+
+def test_pager_refusals():
+    from vllm_expert_pager.adapters import AdapterPager
+
+    t = torch.bfloat16
+    pager = AdapterPager(4, 2, 5, 16, 8, t, DEV)
+    try:
+        assert pager.rank == 8
+        y, x = torch.ones((3, 8), dtype=t, device=DEV), torch.ones((3, 16), dtype=t, device=DEV)
+        with pytest.raises(RuntimeError, match="page the step"):
+            pager.add(y, x, torch.zeros((3,), dtype=torch.int32, device=DEV))
+        for i in (-1, 4):
+            with pytest.raises(ValueError, match="adapter must be in"):
+                pager.write(i, torch.zeros((2, 16), dtype=t), torch.zeros((8, 2), dtype=t))
+        for a, b in ((torch.zeros((9, 16)), torch.zeros((8, 9))),
+                     (torch.zeros((2, 15)), torch.zeros((8, 2))),
+                     (torch.zeros((2, 16)), torch.zeros((8, 3))),
+                     (torch.zeros((16,)), torch.zeros((8, 1)))):
+            with pytest.raises(ValueError, match="expected a"):
+                pager.write(0, a.to(t), b.to(t))
+        with pytest.raises(ValueError, match="of this pager are"):
+            pager.write(0, torch.zeros((2, 16)), torch.zeros((8, 2)))
+        with pytest.raises(ValueError, match="CUDA tensor"):
+            pager.page(torch.zeros((1,), dtype=torch.int32))
+        # Never written: zero.  An empty step pages nothing.
+        pager.page(torch.tensor([1, 2], dtype=torch.int32, device=DEV))
+        assert torch.equal(pager.add(y, x, torch.tensor([1, 2, 1], device=DEV),
+                                     out=torch.empty_like(y)), y)
+        pager.page(torch.zeros((0,), dtype=torch.int64, device=DEV))
+    finally:
+        pager.release()
+        pager.release()

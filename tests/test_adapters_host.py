@@ -12,10 +12,10 @@ P = ctypes.addressof(BUF)
 
 
 def xp_add(x=P, xs=64, y=P, ys=32, out=P, os=32, dtype=1, M=4, H=64, N=32, r=8, a=P, b=P, slots=4,
-           scale=None, ids=P, ids_bytes=4, slot_of=None, adapters_=0, scratch=None,
+           scale=None, ids=P, ids_bytes=4, slot_of=None, slot_bytes=4, adapters_=0, scratch=None,
            scratch_bytes=0):
     return native.lib().xp_add_low_rank(x, xs, y, ys, out, os, dtype, M, H, N, r, a, b, slots,
-                                        scale, ids, ids_bytes, slot_of, adapters_, scratch,
+                                        scale, ids, ids_bytes, slot_of, slot_bytes, adapters_, scratch,
                                         scratch_bytes, None)
 
 
@@ -25,7 +25,8 @@ def xp_add(x=P, xs=64, y=P, ys=32, out=P, os=32, dtype=1, M=4, H=64, N=32, r=8, 
     ({"r": 0}, native.XP_EINVAL), ({"r": 129}, native.XP_ERANGE),
     ({"slots": 0}, native.XP_EINVAL), ({"slots": 8193}, native.XP_ERANGE),
     ({"H": 1 << 31}, native.XP_ERANGE), ({"N": 1 << 31}, native.XP_ERANGE), ({"M": (1 << 26) + 1}, native.XP_ERANGE),
-    ({"ids_bytes": 2}, native.XP_EINVAL), ({"xs": -1}, native.XP_EINVAL),
+    ({"ids_bytes": 2}, native.XP_EINVAL), ({"slot_of": P, "slot_bytes": 2}, native.XP_EINVAL),
+    ({"xs": -1}, native.XP_EINVAL),
     ({"ys": -1}, native.XP_EINVAL), ({"os": 31}, native.XP_EINVAL),
     ({"adapters_": -1}, native.XP_EINVAL), ({"x": None}, native.XP_EINVAL),
     ({"y": None}, native.XP_EINVAL), ({"out": None}, native.XP_EINVAL),
@@ -86,7 +87,8 @@ def operands(M=6, H=16, N=24, r=4, S=3, t=torch.bfloat16):
     (dict(ids=torch.zeros((6,))), "ids must be"),
     (dict(scale=torch.zeros((4,))), "scale must be"),
     (dict(scale=torch.zeros((3,), dtype=torch.float64)), "scale must be"),
-    (dict(slot_map=torch.zeros((9,), dtype=torch.int64)), "slot_map must be"),
+    (dict(slot_map=torch.zeros((9,), dtype=torch.int16)), "slot_map must be"),
+    (dict(slot_map=torch.zeros((9, 1), dtype=torch.int32)), "slot_map must be"),
     (dict(a=torch.zeros((3, 16, 4), dtype=torch.bfloat16).transpose(1, 2)), "contiguous"),
     (dict(out=torch.zeros((24, 6), dtype=torch.bfloat16).t()), "rows of out"),
     (dict(out=torch.zeros((1, 24), dtype=torch.bfloat16).expand(6, 24)), "rows of out"),
@@ -136,3 +138,21 @@ def test_columns_of_one_buffer_do_not_overlap():
     assert share(wide[:, 30:50], wide[:, 10:31])
     assert share(wide[:3], wide[2:5]) and share(wide, wide)
     assert not share(wide[:3], wide[3:])
+
+
+@pytest.mark.parametrize("args, words", [
+    ((0, 1, 8, 16, 16, torch.bfloat16), "num_adapters"),
+    ((4097, 1, 8, 16, 16, torch.bfloat16), "num_adapters"),
+    ((4, 0, 8, 16, 16, torch.bfloat16), "slots must be"),
+    ((4, 5, 8, 16, 16, torch.bfloat16), "slots must be"),
+    ((4000, 2049, 8, 16, 16, torch.bfloat16), "slots must be"),
+    ((4, 2, 0, 16, 16, torch.bfloat16), "the rank must be"),
+    ((4, 2, 129, 16, 16, torch.bfloat16), "the rank must be"),
+    ((4, 2, 8, 0, 16, torch.bfloat16), "the rank must be"),
+    ((4, 2, 8, 16, 0, torch.bfloat16), "the rank must be"),
+    ((4, 2, 8, 16, 16, torch.float32), "bfloat16 or float16"),
+    ((4, 2, 8, 16, 16, torch.bfloat16), "lives on a CUDA device"),
+])
+def test_pager_refuses_its_arguments(args, words):
+    with pytest.raises(ValueError, match=words):
+        adapters.AdapterPager(*args, torch.device("cpu"))

@@ -55,7 +55,8 @@ struct LowRankArgs {
   const float *scale;
   const void *ids;
   int ids_bytes;
-  const int32_t *slot_of;
+  const void *slot_of;  // NULL: ids are slots
+  int slot_bytes;
   int64_t adapters;
   int vec_x, vec_a, vec_b, vec_y;  // 16-byte accesses to x, A, B, and y with out
   int in_place;
@@ -132,7 +133,7 @@ __device__ __forceinline__ float range_factor(float amax) {
 // The slot of row m, -1 without an adapter.
 __device__ __forceinline__ int slot_of_row(const LowRankArgs &a, int64_t m) {
   int64_t s = load_id(a.ids, a.ids_bytes, m);
-  if (a.slot_of) s = s >= 0 && s < a.adapters ? a.slot_of[s] : -1;
+  if (a.slot_of) s = s >= 0 && s < a.adapters ? load_id(a.slot_of, a.slot_bytes, s) : -1;
   return s >= 0 && s < a.slots ? static_cast<int>(s) : -1;
 }
 
@@ -1523,14 +1524,15 @@ extern "C" int xp_add_low_rank(const void *x, int64_t x_stride, const void *y, i
                                void *out, int64_t out_stride, int dtype, int64_t M, int64_t H,
                                int64_t N, int64_t r, const void *a, const void *b, int64_t slots,
                                const float *scale, const void *ids, int ids_bytes,
-                               const int32_t *slot_of, int64_t adapters, void *scratch,
-                               int64_t scratch_bytes, void *stream) {
+                               const void *slot_of, int slot_bytes, int64_t adapters,
+                               void *scratch, int64_t scratch_bytes, void *stream) {
   if (dtype != XP_BF16 && dtype != XP_F16) return XP_EINVAL;
   if (M < 0 || H < 1 || N < 1 || r < 1 || slots < 1 || adapters < 0) return XP_EINVAL;
   if (M > XP_MAX_TOKENS || r > XP_MAX_RANK || slots > XP_MAX_ADAPTER_SLOTS || H > INT32_MAX ||
       N > INT32_MAX)
     return XP_ERANGE;
   if (ids_bytes != 4 && ids_bytes != 8) return XP_EINVAL;
+  if (slot_of && slot_bytes != 4 && slot_bytes != 8) return XP_EINVAL;
   if (x_stride < 0 || y_stride < 0 || (M > 1 && out_stride < N)) return XP_EINVAL;
   if (M == 0) return XP_OK;
   if (!x || !y || !out || !a || !b || !ids) return XP_EINVAL;
@@ -1539,7 +1541,7 @@ extern "C" int xp_add_low_rank(const void *x, int64_t x_stride, const void *y, i
     return XP_EINVAL;
   LowRankArgs p{x, y, out, x_stride, y_stride, out_stride, M, H, N,
                 static_cast<int>(r), static_cast<int>(slots), a, b, scale, ids, ids_bytes, slot_of,
-                adapters};
+                slot_bytes, adapters};
   p.vec_x = aligned(x, 16) && x_stride % 8 == 0;
   p.vec_a = aligned(a, 16) && H % 8 == 0;
   p.vec_b = aligned(b, 16) && r % 8 == 0;

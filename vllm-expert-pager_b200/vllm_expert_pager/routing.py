@@ -157,8 +157,8 @@ def route(logits: torch.Tensor, topk: int, *, renormalize: bool = True,
 
     The experts with the largest logits, in descending order (equal logits: the
     lower expert first); a logit of -inf closes its expert, and where fewer than
-    ``topk`` are open the remaining ids are -1 and their weights 0 (the pager
-    and the MoE ignore them).  ``weights`` are the softmax probabilities of the
+    ``topk`` are open the remaining ids are -1 and their weights 0 (the pager's
+    tables ignore ids out of range).  ``weights`` are the softmax probabilities of the
     chosen experts, divided by their sum with ``renormalize``.  A NaN logit is
     chosen first and makes its token's weights NaN.  ``valid`` (bool ``[T]``)
     marks the rows that hold a token: the others get ids -1 and weights 0, and
