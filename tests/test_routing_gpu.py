@@ -118,8 +118,8 @@ def check_route(logits, K, renormalize, valid=None, train=True, seed=1):
     if not train:
         assert r.loss is None
         return r
-    # P adds up a warp's tokens, the CTA's 16 warps and 296 CTAs at most.
-    adds = T / (296 * 8) + 16 + 296
+    # P adds up a warp's tokens, the CTA's 16 warps and 444 CTAs at most.
+    adds = T / (148 * 8) + 16 + 444
     finite = torch.where(p > 1e-38, x.abs(), 0.0)  # smaller ones are below every bound
     rel = (steps(finite.max() if T else torch.zeros(()), E) + adds) * STEP
     close(r.loss.detach(), loss, float(rel) * loss + 1e-300)
@@ -268,7 +268,7 @@ def test_balance_loss_matches_the_definition(dtype, T, E, K, ids_dtype):
     leaf = logits.detach().requires_grad_()
     loss, got = routing.balance_loss(leaf, ids.to(ids_dtype), valid=valid)
     assert torch.equal(got, counts)
-    bound = (steps(x.abs().max(), E) + T / (296 * 8) + 312) * STEP
+    bound = (steps(x.abs().max(), E) + T / (148 * 8) + 460) * STEP
     close(loss.detach(), want, float(bound) * want + 1e-300)
     with torch.no_grad():
         again, _ = routing.balance_loss(leaf, ids.to(ids_dtype), valid=valid)

@@ -32,8 +32,16 @@ constexpr unsigned kFull = 0xffffffffu;
 // Key of -inf (see key_of): entries at or below it cannot be chosen.
 constexpr uint32_t kKeyNegInf = 0x007fffffu;
 constexpr int kSumCtas = 8;       // CTAs (one cluster) of the sum over CTAs
-constexpr int kSumThreads = 256;
-constexpr int kMaxCtas = 296;     // CTAs of the forward kernel: 2 for each of 148 SMs
+constexpr int kSumThreads = 1024;
+constexpr int kMaxCtas = 444;     // most CTAs of the forward kernel (3 for each of 148 SMs)
+
+// Threads of a CTA of the forward kernel and CTAs on an SM, by the values per lane:
+// what the registers allow without spills.
+constexpr int forward_threads(int vpl) { return vpl <= 8 ? 512 : 256; }
+constexpr int forward_blocks(int vpl) { return vpl <= 8 ? 2 : (vpl <= 16 ? 3 : (vpl <= 32 ? 2 : 1)); }
+constexpr int values_per_lane(int64_t E) {
+  return E <= 64 ? 2 : (E <= 256 ? 8 : (E <= 512 ? 16 : (E <= 1024 ? 32 : 128)));
+}
 
 // A float's order as an unsigned integer; NaN above +inf, -0 equal to +0.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -95,21 +103,34 @@ struct Row {
     return ((i / kV) * 32 + lane) * kV + i % kV;
   }
 
-  static __device__ __forceinline__ void load(const T *row, int E, int lane, float *v) {
+  // A row in two steps, so that the next one can be on its way.
+  struct Raw {
+    uint4 q[VEC ? VPL / kV : 1];
+    T x[VEC ? 1 : VPL];
+  };
+
+  static __device__ __forceinline__ void fetch(const T *row, int E, int lane, Raw &raw) {
 #pragma unroll
     for (int c = 0; c < VPL / kV; ++c) {
       const int e = (c * 32 + lane) * kV;
-      if constexpr (VEC) {
-        if (e < E) {
-          const uint4 q = __ldg(reinterpret_cast<const uint4 *>(row + e));
+      if (e >= E) continue;
+      if constexpr (VEC)
+        raw.q[c] = __ldg(reinterpret_cast<const uint4 *>(row + e));
+      else
+        raw.x[c] = row[e];
+    }
+  }
+
+  static __device__ __forceinline__ void open(const Raw &raw, int E, int lane, float *v) {
 #pragma unroll
-          for (int i = 0; i < kV; ++i) v[c * kV + i] = Pack<T>::at(q, i);
-        } else {
+    for (int c = 0; c < VPL / kV; ++c) {
+      const bool in = (c * 32 + lane) * kV < E;
 #pragma unroll
-          for (int i = 0; i < kV; ++i) v[c * kV + i] = -INFINITY;
-        }
-      } else {
-        v[c] = e < E ? widen(row[e]) : -INFINITY;
+      for (int i = 0; i < kV; ++i) {
+        if constexpr (VEC)
+          v[c * kV + i] = in ? Pack<T>::at(raw.q[c], i) : -INFINITY;
+        else
+          v[c] = in ? widen(raw.x[c]) : -INFINITY;
       }
     }
   }
@@ -131,12 +152,23 @@ struct Row {
   }
 };
 
+// The largest value that is not NaN (-inf: there is none), and whether the row has
+// anything to take a softmax of: a finite value, +inf or NaN.
 template <int VPL>
-__device__ __forceinline__ float row_max(const float *v) {
-  uint32_t k = 0;
+__device__ __forceinline__ float row_max(const float *v, bool *live) {
+  float m = v[0];
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) k = max(k, key_of(v[i]));
-  return of_key(__reduce_max_sync(kFull, k));
+  for (int i = 1; i < VPL; ++i) m = fmaxf(m, v[i]);
+  if (m != m) m = -INFINITY;  // all of this lane's
+  m = of_key(__reduce_max_sync(kFull, key_of(m)));
+  *live = true;
+  if (m == -INFINITY) {  // rare: NaN alone, or nothing
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) nan |= v[i] != v[i];
+    *live = __any_sync(kFull, nan);
+  }
+  return m;
 }
 
 struct ForwardArgs {
@@ -165,7 +197,7 @@ __device__ __forceinline__ float finish(const ForwardArgs &a, int e, float p, in
 }
 
 template <typename T, int VPL, bool VEC>
-__global__ void __launch_bounds__(VPL > 32 ? 256 : 512, VPL <= 16 ? 2 : 1)
+__global__ void __launch_bounds__(forward_threads(VPL), forward_blocks(VPL))
     forward_kernel(const __grid_constant__ ForwardArgs a) {
   using R = Row<T, VPL, VEC>;
   // Rows too long for a second set of registers keep their sums of p in shared
@@ -174,6 +206,7 @@ __global__ void __launch_bounds__(VPL > 32 ? 256 : 512, VPL <= 16 ? 2 : 1)
   extern __shared__ __align__(16) unsigned char smem[];
   const int E = a.E, warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool balance = a.loss != nullptr;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   int *cnt = reinterpret_cast<int *>(smem);               // [E]
   float *sum = reinterpret_cast<float *>(smem) + E;       // [E], or [warps][E]
   __shared__ int tokens;
@@ -193,46 +226,77 @@ __global__ void __launch_bounds__(VPL > 32 ? 256 : 512, VPL <= 16 ? 2 : 1)
     for (int i = 0; i < VPL; ++i) acc[i] = 0.0f;
   }
   int mine = 0;  // tokens of this warp that count
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * warps + warp; t < a.T;
-       t += static_cast<int64_t>(gridDim.x) * warps) {
-    const bool live = !a.valid || a.valid[t];
-    if (!live) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * warps;
+  int64_t t = static_cast<int64_t>(blockIdx.x) * warps + warp;
+  // A token's row is fetched while the one before it is worked on, its flag one
+  // token earlier still.
+  auto counts = [&](int64_t u) { return u < a.T && (!a.valid || a.valid[u]); };
+  auto row_of = [&](int64_t u) { return static_cast<const T *>(a.logits) + u * a.stride; };
+  constexpr bool kAhead = VPL <= 32;
+  typename R::Raw raw;
+  bool live = counts(t), next_live = counts(t + step);
+  if (live) R::fetch(row_of(t), E, lane, raw);
+  for (; t < a.T; t += step) {
+    float v[VPL];
+    const bool here = live;
+    if (here) R::open(raw, E, lane, v);
+    live = next_live;
+    if (kAhead) {
+      next_live = counts(t + 2 * step);
+      if (live) R::fetch(row_of(t + step), E, lane, raw);
+    }
+    if (!here) {
       if (!a.given && lane < a.topk) {
         a.weights[t * a.topk + lane] = 0.0f;
         a.ids[t * a.topk + lane] = -1;
       }
+      if (!kAhead) {
+        next_live = counts(t + 2 * step);
+        if (live) R::fetch(row_of(t + step), E, lane, raw);
+      }
       continue;
     }
     ++mine;
-    float v[VPL];
-    R::load(static_cast<const T *>(a.logits) + t * a.stride, E, lane, v);
-    float m = 0.0f, z = 0.0f;
+    float z = 0.0f;
     if (balance || (!a.given && !a.renormalize)) {
-      m = row_max<VPL>(v);
-      if (m > -INFINITY || m != m) {
+      bool any;
+      const float m = row_max<VPL>(v, &any);
+      if (any) {
+        if constexpr (kAccShared) {
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) z += __expf(v[i] - m);
-        z = warp_sum(z);
-        if (balance) {
-          const float inv = 1.0f / z;
+          for (int i = 0; i < VPL; ++i) z += __expf(v[i] - m);
+          z = warp_sum(z);
+          if (balance) {
+            const float inv = 1.0f / z;
 #pragma unroll
-          for (int i = 0; i < VPL; ++i) {
-            const float p = __expf(v[i] - m) * inv;
-            if constexpr (kAccShared) {
+            for (int i = 0; i < VPL; ++i) {
               const int e = R::expert(i, lane);
-              if (e < E) sum[warp * E + e] += p;
-            } else {
-              acc[i] += p;
+              if (e < E) sum[warp * E + e] += __expf(v[i] - m) * inv;
             }
+          }
+        } else {
+          float p[VPL];
+#pragma unroll
+          for (int i = 0; i < VPL; ++i) z += p[i] = __expf(v[i] - m);
+          z = warp_sum(z);
+          if (balance) {
+            const float inv = 1.0f / z;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) acc[i] += p[i] * inv;
           }
         }
       }
+    }
+    if (!kAhead) {
+      // (Two rows do not fit the registers; the values are read again below.)
+      next_live = counts(t + 2 * step);
     }
     if (a.given) {
       for (int j = lane; j < a.topk; j += 32) {
         const int64_t id = load_id(a.given, a.given_bytes, t * a.topk + j);
         if (id >= 0 && id < E) atomicAdd(&cnt[id], 1);
       }
+      if (!kAhead && live) R::fetch(row_of(t + step), E, lane, raw);
       continue;
     }
     uint32_t key[VPL], best = 0;
@@ -248,7 +312,9 @@ __global__ void __launch_bounds__(VPL > 32 ? 256 : 512, VPL <= 16 ? 2 : 1)
       const uint32_t top = __reduce_max_sync(kFull, best);
       if (top <= kKeyNegInf) break;
       const unsigned claim = best == top ? static_cast<unsigned>(at) : kFull;
-      const unsigned win = __reduce_min_sync(kFull, claim);
+      const unsigned who = __ballot_sync(kFull, best == top);
+      const unsigned win = (who & (who - 1)) ? __reduce_min_sync(kFull, claim)
+                                             : __shfl_sync(kFull, claim, __ffs(who) - 1);
       if (lane == found) my_key = top, my_id = static_cast<int>(win);
       if (claim == win) {  // the owner takes it out and looks for its next one
         best = 0;
@@ -268,6 +334,7 @@ __global__ void __launch_bounds__(VPL > 32 ? 256 : 512, VPL <= 16 ? 2 : 1)
       a.ids[t * a.topk + lane] = my_id;
     }
     if (lane < found) atomicAdd(&cnt[my_id], 1);
+    if (!kAhead && live) R::fetch(row_of(t + step), E, lane, raw);
   }
 
   if (lane == 0 && mine) atomicAdd(&tokens, mine);
@@ -326,30 +393,36 @@ __global__ void __cluster_dims__(kSumCtas, 1, 1) __launch_bounds__(kSumThreads)
   const bool balance = a.loss != nullptr;
   if (tid == 0) tokens = 0;
   __syncthreads();
-  int n = 0;
-  for (int r = tid; r < rows; r += kSumThreads) n += a.part_n[r];
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the forward kernel's end
+  int n = tid < rows ? a.part_n[tid] : 0;
   n = __reduce_add_sync(kFull, n);
   if (lane == 0) atomicAdd(&tokens, n);
   __syncthreads();
   n = tokens;
   float loss = 0.0f;
   constexpr int kCols = 32, kGroups = kSumThreads / kCols;
+  constexpr int kEach = (kMaxCtas + kGroups - 1) / kGroups;
   for (int e0 = blockIdx.x * kCols; e0 < E; e0 += kSumCtas * kCols) {
     const int e = e0 + lane;
+    float q[kEach];
+    int d[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {  // all of a thread's loads under way at once
+      const int r = warp + i * kGroups;
+      const bool in = e < E && r < rows;
+      d[i] = in ? a.part_c[static_cast<int64_t>(r) * E + e] : 0;
+      q[i] = in && balance ? a.part_p[static_cast<int64_t>(r) * E + e] : 0.0f;
+    }
     float p = 0.0f;
     int c = 0;
-    if (e < E) {
-#pragma unroll 4
-      for (int r = warp; r < rows; r += kGroups) {
-        c += a.part_c[static_cast<int64_t>(r) * E + e];
-        if (balance) p += a.part_p[static_cast<int64_t>(r) * E + e];
-      }
-    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) p += q[i], c += d[i];
     __syncthreads();
     sp[tid] = p;
     sc[tid] = c;
     __syncthreads();
     if (warp == 0 && e < E) {
+#pragma unroll 8
       for (int g = 1; g < kGroups; ++g) p += sp[g * kCols + lane], c += sc[g * kCols + lane];
       loss += finish(a, e, p, c, n);
     }
@@ -401,18 +474,24 @@ __global__ void __launch_bounds__(256, VPL <= 16 ? 4 : (VPL <= 32 ? 2 : 1))
       for (int e = lane; e < E; e += 32) sel[e] = 0.0f;
   }
   __syncthreads();
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * warps + warp; t < a.T;
-       t += static_cast<int64_t>(gridDim.x) * warps) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * warps;
+  int64_t t = static_cast<int64_t>(blockIdx.x) * warps + warp;
+  auto counts = [&](int64_t u) { return u < a.T && (!a.valid || a.valid[u]); };
+  auto row_of = [&](int64_t u) { return static_cast<const T *>(a.logits) + u * a.stride; };
+  typename R::Raw raw;
+  bool now = counts(t), next = counts(t + step);
+  if (now) R::fetch(row_of(t), E, lane, raw);
+  for (; t < a.T; t += step) {
     float v[VPL];
     T *out = static_cast<T *>(a.grad) + t * E;
-    const T *row = static_cast<const T *>(a.logits) + t * a.stride;
-    bool live = !a.valid || a.valid[t];
+    const T *row = row_of(t);
+    bool live = now;
+    if (live) R::open(raw, E, lane, v);
+    now = next;
+    next = counts(t + 2 * step);
+    if (now) R::fetch(row_of(t + step), E, lane, raw);  // the next row, meanwhile
     float m = 0.0f;
-    if (live) {
-      R::load(row, E, lane, v);
-      m = row_max<VPL>(v);
-      live = m > -INFINITY || m != m;
-    }
+    if (live) m = row_max<VPL>(v, &live);
     if (!live) {
 #pragma unroll
       for (int i = 0; i < VPL; ++i) v[i] = 0.0f;
@@ -476,18 +555,18 @@ int set_smem(const void *fn, size_t bytes) {
   return err == cudaSuccess ? XP_OK : static_cast<int>(err);
 }
 
-// CTAs and threads of the forward kernel.
-int forward_threads(int64_t E) { return E > 1024 ? 256 : 512; }
+// CTAs of the forward kernel.
 int64_t forward_ctas(int64_t T, int64_t E) {
-  const int64_t warps = forward_threads(E) / 32;
+  const int vpl = values_per_lane(E);
+  const int64_t warps = forward_threads(vpl) / 32, most = 148 * forward_blocks(vpl);
   const int64_t ctas = (T + warps - 1) / warps;
-  return ctas < 1 ? 1 : (ctas < kMaxCtas ? ctas : kMaxCtas);
+  return ctas < 1 ? 1 : (ctas < most ? ctas : most);
 }
 
 template <typename T, int VPL, bool VEC>
 int launch_forward(const ForwardArgs &a, cudaStream_t s) {
   auto fn = forward_kernel<T, VPL, VEC>;
-  const int threads = forward_threads(a.E);
+  const int threads = forward_threads(VPL);
   const int64_t ctas = forward_ctas(a.T, a.E);
   const int rows = 1 + (a.loss ? (VPL > 32 ? threads / 32 : 1) : 0);
   const size_t smem = sizeof(float) * a.E * rows;
@@ -496,8 +575,18 @@ int launch_forward(const ForwardArgs &a, cudaStream_t s) {
   fn<<<static_cast<unsigned>(ctas), threads, smem, s>>>(a);
   rc = launch_status();
   if (rc || ctas == 1) return rc;
-  sum_kernel<<<kSumCtas, kSumThreads, 0, s>>>(a, static_cast<int>(ctas));
-  return launch_status();
+  // The sum's launch overlaps the forward kernel's end (it waits for it itself).
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kSumCtas);
+  cfg.blockDim = dim3(kSumThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t err = cudaLaunchKernelEx(&cfg, sum_kernel, a, static_cast<int>(ctas));
+  return err == cudaSuccess ? launch_status() : static_cast<int>(err);
 }
 
 template <typename T, int VPL, bool VEC>
@@ -520,17 +609,18 @@ int dispatch(const Args &a, bool vec, cudaStream_t s) {
   constexpr int kN = Pack<T>::kN;
   const int E = a.E;
   vec = vec && E % kN == 0;
-  if (E <= 64) return Launch<T, 2, false>::go(a, s);
-  if (vec) {
-    if (E <= 256) return Launch<T, 8, true>::go(a, s);
-    if (E <= 512) return Launch<T, 16, true>::go(a, s);
-    if (E <= 1024) return Launch<T, 32, true>::go(a, s);
-    return Launch<T, 128, true>::go(a, s);
+  switch (values_per_lane(E)) {
+    case 2:
+      return Launch<T, 2, false>::go(a, s);
+    case 8:
+      return vec ? Launch<T, 8, true>::go(a, s) : Launch<T, 8, false>::go(a, s);
+    case 16:
+      return vec ? Launch<T, 16, true>::go(a, s) : Launch<T, 16, false>::go(a, s);
+    case 32:
+      return vec ? Launch<T, 32, true>::go(a, s) : Launch<T, 32, false>::go(a, s);
+    default:
+      return vec ? Launch<T, 128, true>::go(a, s) : Launch<T, 128, false>::go(a, s);
   }
-  if (E <= 256) return Launch<T, 8, false>::go(a, s);
-  if (E <= 512) return Launch<T, 16, false>::go(a, s);
-  if (E <= 1024) return Launch<T, 32, false>::go(a, s);
-  return Launch<T, 128, false>::go(a, s);
 }
 
 template <typename T, int VPL, bool VEC>
