@@ -334,14 +334,15 @@ int xp_balance(const void *logits, int dtype, int64_t T, int64_t E, int64_t stri
                int64_t scratch_bytes, void *stream);
 
 /* grad[T][E] (contiguous, dtype as logits): the gradient of the logits.
- * grad_weights[T][topk] (NULL: none) is the gradient of xp_route's weights for
- * the ids that it wrote; grad_loss (NULL: none) points at the gradient of the
+ * grad_weights[T][topk] (NULL: none) is the gradient of xp_route's weights, with
+ * the ids and weights that it wrote; grad_loss (NULL: none) points at the gradient of the
  * loss, with counts and tokens as the forward call wrote them (tokens may be
  * NULL when valid is: all rows are tokens).  Rows that are not valid
  * get zeros. */
 int xp_route_backward(const void *logits, int dtype, int64_t T, int64_t E, int64_t stride,
-                      const uint8_t *valid, const int32_t *ids, int64_t topk, int renormalize,
-                      const float *grad_weights, const int64_t *counts, const int64_t *tokens,
+                      const uint8_t *valid, const int32_t *ids, const float *weights,
+                      int64_t topk, int renormalize, const float *grad_weights,
+                      const int64_t *counts, const int64_t *tokens,
                       const float *grad_loss, void *grad, void *stream);
 
 /* ---- low-rank adapters of many requests ----

@@ -27,9 +27,9 @@ def xp_balance(logits=P, dtype=0, T=4, E=8, stride=8, valid=None, ids=P, ids_byt
                                    counts, tokens, loss, scratch, scratch_bytes, None)
 
 
-def xp_backward(logits=P, dtype=0, T=4, E=8, stride=8, valid=None, ids=P, topk=2, renorm=1,
+def xp_backward(logits=P, dtype=0, T=4, E=8, stride=8, valid=None, ids=P, weights=P, topk=2, renorm=1,
                 grad_weights=P, counts=P, tokens=P, grad_loss=P, grad=P):
-    return native.lib().xp_route_backward(logits, dtype, T, E, stride, valid, ids, topk, renorm,
+    return native.lib().xp_route_backward(logits, dtype, T, E, stride, valid, ids, weights, topk, renorm,
                                           grad_weights, counts, tokens, grad_loss, grad, None)
 
 
@@ -63,6 +63,7 @@ def test_balance_checks_its_arguments(change, status):
 
 @pytest.mark.parametrize("change, status", [
     ({"topk": 40}, native.XP_ERANGE), ({"ids": None}, native.XP_EINVAL),
+    ({"weights": None}, native.XP_EINVAL),
     ({"grad": None}, native.XP_EINVAL), ({"counts": None}, native.XP_EINVAL),
     ({"tokens": None, "valid": P}, native.XP_EINVAL), ({"logits": None}, native.XP_EINVAL),
     ({"E": 0}, native.XP_EINVAL), ({"T": 0}, native.XP_OK),

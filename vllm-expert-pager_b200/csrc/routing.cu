@@ -13,13 +13,17 @@
 //
 // One warp owns a token: the logits stay in registers (VPL a lane), maxima go
 // through one redux instruction on order-preserving integer keys, and a token's
-// reads are whole 16-byte vectors.  Sums over tokens (P, c) are kept per lane
+// reads are whole 16-byte vectors.  For the choice a lane's logits become integers
+// that hold their order and their expert (see Choice), sorted in registers; each of
+// the k steps then takes the largest first one of the lanes' runs.  Sums over tokens (P, c) are kept per lane
 // over a warp's tokens, added over the CTA's warps in their order, and over the
 // CTAs in theirs by a second small launch: no atomics on floats, so the loss does
 // not depend on the order in which CTAs run.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -29,8 +33,6 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr unsigned kFull = 0xffffffffu;
-// Key of -inf (see key_of): entries at or below it cannot be chosen.
-constexpr uint32_t kKeyNegInf = 0x007fffffu;
 constexpr int kSumCtas = 8;       // CTAs (one cluster) of the sum over CTAs
 constexpr int kSumThreads = 1024;
 constexpr int kMaxCtas = 444;     // most CTAs of the forward kernel (3 for each of 148 SMs)
@@ -39,6 +41,10 @@ constexpr int kMaxCtas = 444;     // most CTAs of the forward kernel (3 for each
 // what the registers allow without spills.
 constexpr int forward_threads(int vpl) { return vpl <= 8 ? 512 : 256; }
 constexpr int forward_blocks(int vpl) { return vpl <= 8 ? 2 : (vpl <= 16 ? 3 : (vpl <= 32 ? 2 : 1)); }
+constexpr int kBackThreads = 256;  // the backward kernel's
+constexpr int backward_blocks(int vpl) {
+  return vpl <= 8 ? 4 : (vpl <= 16 ? 3 : (vpl <= 32 ? 2 : 1));
+}
 constexpr int values_per_lane(int64_t E) {
   return E <= 64 ? 2 : (E <= 256 ? 8 : (E <= 512 ? 16 : (E <= 1024 ? 32 : 128)));
 }
@@ -53,16 +59,93 @@ __device__ __forceinline__ float of_key(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
+// A logit and its expert as one integer: larger logits above smaller ones, of equal
+// ones the lower expert above; 0 is nothing, kOpen the least that can be chosen
+// (above -inf).  16-bit logits need 16 bits for their order, so that one 32-bit
+// maximum decides; 32-bit logits take 64 bits and two.
+template <typename T>
+struct Choice {
+  using K = uint32_t;
+  static constexpr bool kHalf = std::is_same<T, __half>::value;
+  static constexpr K kOpen = (kHalf ? 0x0400u : 0x0080u) << 16;
+  static __device__ __forceinline__ K make(float x, int e) {
+    x = x + 0.0f;  // -0 equals 0
+    uint32_t u = kHalf ? static_cast<uint32_t>(__half_as_ushort(__float2half_rn(x))) << 16
+                       : __float_as_uint(x);
+    if (x != x) u = 0x7fff0000u;
+    u ^= static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u;
+    return (u & 0xffff0000u) | (0xffffu - e);
+  }
+  static __device__ __forceinline__ int expert(K k) { return 0xffff - static_cast<int>(k & 0xffff); }
+  static __device__ __forceinline__ float logit(K k) {
+    const uint32_t u = (k & 0x80000000u ? k ^ 0x80000000u : ~k) & 0xffff0000u;
+    return kHalf ? __half2float(__ushort_as_half(static_cast<unsigned short>(u >> 16)))
+                 : __uint_as_float(u);
+  }
+  static __device__ __forceinline__ K warp_max(K k) { return __reduce_max_sync(kFull, k); }
+};
+
+template <>
+struct Choice<float> {
+  using K = uint64_t;
+  static constexpr K kOpen = 0x00800000ull << 32;
+  static __device__ __forceinline__ K make(float x, int e) {
+    return static_cast<K>(key_of(x)) << 32 | (0xffffffffu - static_cast<uint32_t>(e));
+  }
+  static __device__ __forceinline__ int expert(K k) {
+    return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k));
+  }
+  static __device__ __forceinline__ float logit(K k) {
+    return of_key(static_cast<uint32_t>(k >> 32));
+  }
+  static __device__ __forceinline__ K warp_max(K k) {
+    const uint32_t hi = static_cast<uint32_t>(k >> 32), top = __reduce_max_sync(kFull, hi);
+    const unsigned who = __ballot_sync(kFull, hi == top);
+    const uint32_t lo = static_cast<uint32_t>(k);
+    // Equal logits in several lanes: the lower expert.
+    const uint32_t low = (who & (who - 1)) ? __reduce_max_sync(kFull, hi == top ? lo : 0u)
+                                           : __shfl_sync(kFull, lo, __ffs(who) - 1);
+    return static_cast<K>(top) << 32 | low;
+  }
+};
+
+// Sorts n values in descending order (Batcher's odd-even merges; unrolled whole).
+template <int n, typename K>
+__device__ __forceinline__ void sort_down(K (&k)[n]) {
+#pragma unroll
+  for (int p = 1; p < n; p *= 2)
+#pragma unroll
+    for (int d = p; d >= 1; d /= 2)
+#pragma unroll
+      for (int j = d % p; j + d < n; j += 2 * d)
+#pragma unroll
+        for (int i = 0; i < d; ++i)
+          if (i + j + d < n && (i + j) / (2 * p) == (i + j + d) / (2 * p)) {
+            const K u = k[i + j], w = k[i + j + d];
+            k[i + j] = u > w ? u : w;
+            k[i + j + d] = u > w ? w : u;
+          }
+}
+
 __device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(kFull, x, o);
   return x;
 }
 
+// exp(x) for x <= 0 by the hardware's power of two (2 steps of 2^-23, and as much for
+// each unit of x from the rounding of x log2 e); below 2^-126 it is 0.
+__device__ __forceinline__ float exp_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
+
 template <typename T>
 struct Pack;  // 16 bytes of logits
 template <>
 struct Pack<float> {
+  static constexpr uint32_t kMinusInf = 0xff800000u;
   static constexpr int kN = 4;
   static __device__ __forceinline__ float at(const uint4 &q, int i) {
     return __uint_as_float((&q.x)[i]);
@@ -70,6 +153,7 @@ struct Pack<float> {
 };
 template <>
 struct Pack<__nv_bfloat16> {
+  static constexpr uint32_t kMinusInf = 0xff80ff80u;
   static constexpr int kN = 8;
   static __device__ __forceinline__ float at(const uint4 &q, int i) {
     const uint32_t w = (&q.x)[i >> 1];
@@ -78,6 +162,7 @@ struct Pack<__nv_bfloat16> {
 };
 template <>
 struct Pack<__half> {
+  static constexpr uint32_t kMinusInf = 0xfc00fc00u;
   static constexpr int kN = 8;
   static __device__ __forceinline__ float at(const uint4 &q, int i) {
     const uint32_t w = (&q.x)[i >> 1];
@@ -103,10 +188,22 @@ struct Row {
     return ((i / kV) * 32 + lane) * kV + i % kV;
   }
 
-  // A row in two steps, so that the next one can be on its way.
+  // A row in two steps, so that the next one can be on its way.  Places past the
+  // row's end hold -inf from the start; no fetch touches them.
   struct Raw {
     uint4 q[VEC ? VPL / kV : 1];
     T x[VEC ? 1 : VPL];
+
+    __device__ __forceinline__ Raw() {
+      const uint32_t w = Pack<T>::kMinusInf;
+      if constexpr (VEC) {
+#pragma unroll
+        for (int c = 0; c < VPL / kV; ++c) q[c] = make_uint4(w, w, w, w);
+      } else {
+#pragma unroll
+        for (int c = 0; c < VPL; ++c) narrow(&x[c], -INFINITY);
+      }
+    }
   };
 
   static __device__ __forceinline__ void fetch(const T *row, int E, int lane, Raw &raw) {
@@ -121,16 +218,27 @@ struct Row {
     }
   }
 
-  static __device__ __forceinline__ void open(const Raw &raw, int E, int lane, float *v) {
+  static __device__ __forceinline__ void open(const Raw &raw, float *v) {
 #pragma unroll
-    for (int c = 0; c < VPL / kV; ++c) {
-      const bool in = (c * 32 + lane) * kV < E;
+    for (int i = 0; i < VPL; ++i) {
+      if constexpr (VEC)
+        v[i] = Pack<T>::at(raw.q[i / kV], i % kV);
+      else
+        v[i] = widen(raw.x[i]);
+    }
+  }
+
+  // The lane's values of a row of floats in shared memory (16-byte aligned; places
+  // past its end are read too, as far as the row is padded).
+  static __device__ __forceinline__ void gather(const float *row, int lane, float *v) {
 #pragma unroll
-      for (int i = 0; i < kV; ++i) {
-        if constexpr (VEC)
-          v[c * kV + i] = in ? Pack<T>::at(raw.q[c], i) : -INFINITY;
-        else
-          v[c] = in ? widen(raw.x[c]) : -INFINITY;
+    for (int i = 0; i < VPL; i += (VEC ? 4 : 1)) {
+      const float *p = row + expert(i, lane);
+      if constexpr (VEC) {
+        const float4 q = *reinterpret_cast<const float4 *>(p);
+        v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
+      } else {
+        v[i] = *p;
       }
     }
   }
@@ -196,7 +304,8 @@ __device__ __forceinline__ float finish(const ForwardArgs &a, int e, float p, in
   return (static_cast<float>(c) / (static_cast<float>(n) * a.topk)) * (p / n);
 }
 
-template <typename T, int VPL, bool VEC>
+// kGiven: the ids were chosen elsewhere.
+template <typename T, int VPL, bool VEC, bool kGiven>
 __global__ void __launch_bounds__(forward_threads(VPL), forward_blocks(VPL))
     forward_kernel(const __grid_constant__ ForwardArgs a) {
   using R = Row<T, VPL, VEC>;
@@ -239,14 +348,14 @@ __global__ void __launch_bounds__(forward_threads(VPL), forward_blocks(VPL))
   for (; t < a.T; t += step) {
     float v[VPL];
     const bool here = live;
-    if (here) R::open(raw, E, lane, v);
+    if (here) R::open(raw, v);
     live = next_live;
     if (kAhead) {
       next_live = counts(t + 2 * step);
       if (live) R::fetch(row_of(t + step), E, lane, raw);
     }
     if (!here) {
-      if (!a.given && lane < a.topk) {
+      if (!kGiven && lane < a.topk) {
         a.weights[t * a.topk + lane] = 0.0f;
         a.ids[t * a.topk + lane] = -1;
       }
@@ -257,27 +366,29 @@ __global__ void __launch_bounds__(forward_threads(VPL), forward_blocks(VPL))
       continue;
     }
     ++mine;
+    int64_t given = -1;  // the first 32 of given ids, on their way during the softmax
+    if (kGiven && lane < a.topk) given = load_id(a.given, a.given_bytes, t * a.topk + lane);
     float z = 0.0f;
-    if (balance || (!a.given && !a.renormalize)) {
+    if (kGiven || balance || !a.renormalize) {
       bool any;
       const float m = row_max<VPL>(v, &any);
       if (any) {
         if constexpr (kAccShared) {
 #pragma unroll
-          for (int i = 0; i < VPL; ++i) z += __expf(v[i] - m);
+          for (int i = 0; i < VPL; ++i) z += exp_fast(v[i] - m);
           z = warp_sum(z);
           if (balance) {
             const float inv = 1.0f / z;
 #pragma unroll
             for (int i = 0; i < VPL; ++i) {
               const int e = R::expert(i, lane);
-              if (e < E) sum[warp * E + e] += __expf(v[i] - m) * inv;
+              if (e < E) sum[warp * E + e] += exp_fast(v[i] - m) * inv;
             }
           }
         } else {
           float p[VPL];
 #pragma unroll
-          for (int i = 0; i < VPL; ++i) z += p[i] = __expf(v[i] - m);
+          for (int i = 0; i < VPL; ++i) z += p[i] = exp_fast(v[i] - m);
           z = warp_sum(z);
           if (balance) {
             const float inv = 1.0f / z;
@@ -291,43 +402,70 @@ __global__ void __launch_bounds__(forward_threads(VPL), forward_blocks(VPL))
       // (Two rows do not fit the registers; the values are read again below.)
       next_live = counts(t + 2 * step);
     }
-    if (a.given) {
+    if constexpr (kGiven) {
       for (int j = lane; j < a.topk; j += 32) {
-        const int64_t id = load_id(a.given, a.given_bytes, t * a.topk + j);
-        if (id >= 0 && id < E) atomicAdd(&cnt[id], 1);
+        if (j >= 32) given = load_id(a.given, a.given_bytes, t * a.topk + j);
+        if (given >= 0 && given < E) atomicAdd(&cnt[given], 1);
       }
       if (!kAhead && live) R::fetch(row_of(t + step), E, lane, raw);
       continue;
     }
-    uint32_t key[VPL], best = 0;
-    int at = 0;
+    // The lanes' choices: sorted where that is cheaper than to look through them
+    // again after each step.  Unsorted 32-bit logits keep the 32 bits of their order
+    // alone (a value's place gives its expert), half the registers.
+    using C = Choice<T>;
+    using K = typename C::K;
+    constexpr bool kWide = sizeof(K) == 8;
+    constexpr bool kSort = VPL <= 8 || (VPL <= 16 && !kWide);
+    using Kept = typename std::conditional<kWide && !kSort, uint32_t, K>::type;
+    Kept all[VPL] = {};
+    K best = 0, mine_k = 0;
+    auto choice = [&](int i) {
+      if constexpr (kWide && !kSort)
+        return all[i] == 0 ? K(0) : static_cast<K>(all[i]) << 32 |
+                                        (0xffffffffu - static_cast<uint32_t>(R::expert(i, lane)));
+      else
+        return all[i];
+    };
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      key[i] = key_of(v[i]);
-      if (key[i] > best) best = key[i], at = R::expert(i, lane);
+      const int e = R::expert(i, lane);
+      if constexpr (kWide && !kSort)
+        all[i] = e < E ? key_of(v[i]) : 0;
+      else
+        all[i] = e < E ? C::make(v[i], e) : 0;
     }
-    uint32_t my_key = 0;
-    int my_id = -1, found = 0;
-    for (; found < a.topk; ++found) {
-      const uint32_t top = __reduce_max_sync(kFull, best);
-      if (top <= kKeyNegInf) break;
-      const unsigned claim = best == top ? static_cast<unsigned>(at) : kFull;
-      const unsigned who = __ballot_sync(kFull, best == top);
-      const unsigned win = (who & (who - 1)) ? __reduce_min_sync(kFull, claim)
-                                             : __shfl_sync(kFull, claim, __ffs(who) - 1);
-      if (lane == found) my_key = top, my_id = static_cast<int>(win);
-      if (claim == win) {  // the owner takes it out and looks for its next one
-        best = 0;
+    if constexpr (kSort) {
+      sort_down<VPL>(all);
+      best = all[0];
+    } else {
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-          const int e = R::expert(i, lane);
-          if (e == static_cast<int>(win)) key[i] = 0;
-          if (key[i] > best) best = key[i], at = e;
+      for (int i = 0; i < VPL; ++i) best = best > choice(i) ? best : choice(i);
+    }
+    int found = 0;
+    for (; found < a.topk; ++found) {
+      const K top = C::warp_max(best);
+      if (top < C::kOpen) break;
+      if (lane == found) mine_k = top;
+      if (best == top) {  // this lane's: on to its next one
+        if constexpr (kSort) {
+#pragma unroll
+          for (int i = 0; i + 1 < VPL; ++i) all[i] = all[i + 1];
+          all[VPL - 1] = 0;
+          best = all[0];
+        } else {
+          best = 0;
+#pragma unroll
+          for (int i = 0; i < VPL; ++i) {
+            if (choice(i) == top) all[i] = 0;
+            best = best > choice(i) ? best : choice(i);
+          }
         }
       }
     }
-    const float l = of_key(my_key), top = __shfl_sync(kFull, l, 0);
-    float w = lane < found ? __expf(l - top) : 0.0f;
+    const int my_id = lane < found ? C::expert(mine_k) : -1;
+    const float l = C::logit(mine_k), top = __shfl_sync(kFull, l, 0);
+    float w = lane < found ? exp_fast(l - top) : 0.0f;
     if (a.renormalize) z = warp_sum(w);
     if (lane < a.topk) {
       a.weights[t * a.topk + lane] = lane < found ? w / z : 0.0f;
@@ -445,7 +583,8 @@ struct BackwardArgs {
   int64_t T, stride;
   int E, topk, renormalize;
   const uint8_t *valid;
-  const int32_t *ids;         // the forward pass's choices (with grad_weights)
+  const int32_t *ids;         // the forward pass's choices and weights (with grad_weights)
+  const float *weights;
   const float *grad_weights;  // NULL: no gradient through the weights
   const int64_t *counts;      // [E] (with grad_loss)
   const int64_t *tokens;
@@ -454,13 +593,14 @@ struct BackwardArgs {
 };
 
 template <typename T, int VPL, bool VEC>
-__global__ void __launch_bounds__(256, VPL <= 16 ? 4 : (VPL <= 32 ? 2 : 1))
+__global__ void __launch_bounds__(kBackThreads, backward_blocks(VPL))
     backward_kernel(const __grid_constant__ BackwardArgs a) {
   using R = Row<T, VPL, VEC>;
   extern __shared__ __align__(16) unsigned char smem[];
   const int E = a.E, warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float *h = reinterpret_cast<float *>(smem);         // [E]: dL/dp of the loss
-  float *sel = h + E + static_cast<int64_t>(warp) * E;  // [E] for each warp: the choices' part
+  constexpr int kRow = 32 * VPL;  // a row and its padding
+  float *h = reinterpret_cast<float *>(smem);  // dL/dp of the loss
+  float *sel = h + kRow + warp * kRow;         // for each warp: the choices' part
   const bool balance = a.grad_loss != nullptr, choices = a.grad_weights != nullptr;
   {
     float s = 0.0f;
@@ -468,28 +608,36 @@ __global__ void __launch_bounds__(256, VPL <= 16 ? 4 : (VPL <= 32 ? 2 : 1))
       const float n = static_cast<float>(a.tokens ? *a.tokens : a.T);
       if (n > 0.0f) s = *a.grad_loss * E / n / (n * a.topk);
     }
-    for (int e = threadIdx.x; e < E; e += blockDim.x)
-      h[e] = balance ? s * static_cast<float>(a.counts[e]) : 0.0f;
+    for (int e = threadIdx.x; e < kRow; e += blockDim.x)
+      h[e] = balance && e < E ? s * static_cast<float>(a.counts[e]) : 0.0f;
     if (choices)
-      for (int e = lane; e < E; e += 32) sel[e] = 0.0f;
+      for (int e = lane; e < kRow; e += 32) sel[e] = 0.0f;
   }
   __syncthreads();
   const int64_t step = static_cast<int64_t>(gridDim.x) * warps;
   int64_t t = static_cast<int64_t>(blockIdx.x) * warps + warp;
   auto counts = [&](int64_t u) { return u < a.T && (!a.valid || a.valid[u]); };
   auto row_of = [&](int64_t u) { return static_cast<const T *>(a.logits) + u * a.stride; };
+  constexpr bool kAhead = VPL <= 32;  // two rows fit the registers
   typename R::Raw raw;
   bool now = counts(t), next = counts(t + step);
-  if (now) R::fetch(row_of(t), E, lane, raw);
+  if (kAhead && now) R::fetch(row_of(t), E, lane, raw);
   for (; t < a.T; t += step) {
     float v[VPL];
     T *out = static_cast<T *>(a.grad) + t * E;
-    const T *row = row_of(t);
     bool live = now;
-    if (live) R::open(raw, E, lane, v);
+    if (!kAhead && live) R::fetch(row_of(t), E, lane, raw);
+    if (live) R::open(raw, v);
     now = next;
     next = counts(t + 2 * step);
-    if (now) R::fetch(row_of(t + step), E, lane, raw);  // the next row, meanwhile
+    int id = -1;
+    float w = 0.0f, g = 0.0f;
+    if (choices && lane < a.topk) {
+      id = a.ids[t * a.topk + lane];
+      w = a.weights[t * a.topk + lane];
+      g = a.grad_weights[t * a.topk + lane];
+    }
+    if (kAhead && now) R::fetch(row_of(t + step), E, lane, raw);  // the next row, meanwhile
     float m = 0.0f;
     if (live) m = row_max<VPL>(v, &live);
     if (!live) {
@@ -501,48 +649,58 @@ __global__ void __launch_bounds__(256, VPL <= 16 ? 4 : (VPL <= 32 ? 2 : 1))
     float z = 0.0f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      v[i] = __expf(v[i] - m);
+      v[i] = exp_fast(v[i] - m);
       z += v[i];
     }
     const float inv = 1.0f / warp_sum(z);
     float inner = 0.0f;  // sum_u p_u h_u
+    float u[VPL <= 32 ? VPL : 1];  // h; rows too long for the registers read it twice
+    if constexpr (VPL <= 32) {
+      if (balance) {
+        R::gather(h, lane, u);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) u[i] = 0.0f;
+      }
+    }
+    auto slope = [&](int i) {
+      if constexpr (VPL <= 32)
+        return u[i];
+      else
+        return h[R::expert(i, lane)];
+    };
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      const int e = R::expert(i, lane);
       v[i] *= inv;
-      if (e < E) inner += v[i] * h[e];
+      inner += v[i] * slope(i);
     }
     if (balance) inner = warp_sum(inner);
     if (choices) {
-      int id = -1;
-      float d = 0.0f;
-      if (lane < a.topk) id = a.ids[t * a.topk + lane];
+      // A chosen probability is its weight, or proportional to it.
       const bool has = id >= 0 && id < E;
-      const float g = has ? a.grad_weights[t * a.topk + lane] : 0.0f;
-      float p = has ? __expf(widen(row[id]) - m) : 0.0f;
-      if (a.renormalize) {
-        const float total = warp_sum(p);
-        const float w = has ? p / total : 0.0f;
-        d = w * (g - warp_sum(w * g));
-      } else {
-        d = p * inv * g;
-        inner += warp_sum(d);
-      }
+      float d = has ? w * g : 0.0f;
+      const float both = warp_sum(d);
+      if (a.renormalize)
+        d -= has ? w * both : 0.0f;
+      else
+        inner += both;
       if (has) sel[id] = d;
       __syncwarp();
+      if constexpr (VPL <= 32) {
+        float c[VPL];
+        R::gather(sel, lane, c);
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const int e = R::expert(i, lane);
-        if (e < E) v[i] = v[i] * (h[e] - inner) + sel[e];
+        for (int i = 0; i < VPL; ++i) v[i] = v[i] * (u[i] - inner) + c[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+          v[i] = v[i] * (slope(i) - inner) + sel[R::expert(i, lane)];
       }
       __syncwarp();
       if (has) sel[id] = 0.0f;
     } else {
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const int e = R::expert(i, lane);
-        if (e < E) v[i] *= h[e] - inner;
-      }
+      for (int i = 0; i < VPL; ++i) v[i] *= slope(i) - inner;
     }
     R::store(out, E, lane, v);
   }
@@ -565,7 +723,7 @@ int64_t forward_ctas(int64_t T, int64_t E) {
 
 template <typename T, int VPL, bool VEC>
 int launch_forward(const ForwardArgs &a, cudaStream_t s) {
-  auto fn = forward_kernel<T, VPL, VEC>;
+  auto fn = a.given ? forward_kernel<T, VPL, VEC, true> : forward_kernel<T, VPL, VEC, false>;
   const int threads = forward_threads(VPL);
   const int64_t ctas = forward_ctas(a.T, a.E);
   const int rows = 1 + (a.loss ? (VPL > 32 ? threads / 32 : 1) : 0);
@@ -592,12 +750,12 @@ int launch_forward(const ForwardArgs &a, cudaStream_t s) {
 template <typename T, int VPL, bool VEC>
 int launch_backward(const BackwardArgs &a, cudaStream_t s) {
   auto fn = backward_kernel<T, VPL, VEC>;
-  const int threads = 256;
-  const size_t smem = sizeof(float) * a.E * (1 + (a.grad_weights ? threads / 32 : 0));
+  const int threads = kBackThreads;
+  const size_t smem = sizeof(float) * 32 * VPL * (1 + (a.grad_weights ? threads / 32 : 0));
   int rc = set_smem((const void *)fn, smem);
   if (rc) return rc;
   const int64_t want = (a.T + threads / 32 - 1) / (threads / 32);
-  const int64_t most = 148 * 8;
+  const int64_t most = 148 * backward_blocks(VPL);
   fn<<<static_cast<unsigned>(want < most ? want : most), threads, smem, s>>>(a);
   return launch_status();
 }
@@ -717,18 +875,18 @@ extern "C" int xp_balance(const void *logits, int dtype, int64_t T, int64_t E, i
 
 extern "C" int xp_route_backward(const void *logits, int dtype, int64_t T, int64_t E,
                                  int64_t stride, const uint8_t *valid, const int32_t *ids,
-                                 int64_t topk, int renormalize, const float *grad_weights,
-                                 const int64_t *counts, const int64_t *tokens,
+                                 const float *weights, int64_t topk, int renormalize,
+                                 const float *grad_weights, const int64_t *counts, const int64_t *tokens,
                                  const float *grad_loss, void *grad, void *stream) {
   int rc = check_sizes(dtype, T, E, stride, topk);
   if (rc) return rc;
   if (grad_weights && topk > XP_MAX_TOPK) return XP_ERANGE;
   if (T == 0) return XP_OK;
-  if (!logits || !grad || (grad_weights && !ids) || (grad_loss && !counts) ||
+  if (!logits || !grad || (grad_weights && (!ids || !weights)) || (grad_loss && !counts) ||
       (grad_loss && valid && !tokens))
     return XP_EINVAL;
   BackwardArgs a{logits, T, stride, static_cast<int>(E), static_cast<int>(topk), renormalize,
-                 valid, ids, grad_weights, counts, tokens,
+                 valid, ids, weights, grad_weights, counts, tokens,
                  grad_loss, grad};
   return by_type<BackwardArgs, Backward>(a, dtype, grad, as_stream(stream));
 }

@@ -73,8 +73,8 @@ _SIGNATURES = {
                         _p]),
     "xp_balance": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _p, _i32, _i64, _p, _p, _p, _p, _i64,
                           _p]),
-    "xp_route_backward": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _p, _i64, _i32, _p, _p, _p, _p,
-                                 _p, _p]),
+    "xp_route_backward": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _p, _p, _i64, _i32, _p, _p, _p,
+                                 _p, _p, _p]),
     "xp_low_rank_scratch_bytes": (_i64, [_i64, _i64]),
     "xp_add_low_rank": (_i32, [_p, _i64, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _i64, _p, _p,
                                _i64, _p, _p, _i32, _p, _i32, _i64, _p, _i64, _p]),

@@ -96,7 +96,7 @@ def _once() -> None:
                            "cannot be taken with create_graph=True")
 
 
-def _backward(logits, topk, renormalize, valid, ids, grad_weights, counts, tokens, grad_loss):
+def _backward(logits, topk, renormalize, valid, ids, weights, grad_weights, counts, tokens, grad_loss):
     if grad_weights is not None:
         grad_weights = grad_weights.contiguous()
     T, E = logits.shape
@@ -104,7 +104,7 @@ def _backward(logits, topk, renormalize, valid, ids, grad_weights, counts, token
     ptr = native.ptr
     native.launch(logits.device, "route_backward", native.lib().xp_route_backward,
                   logits.data_ptr(), native.DTYPES[logits.dtype], T, E, logits.stride(0),
-                  ptr(valid), ptr(ids), topk, renormalize, ptr(grad_weights), ptr(counts),
+                  ptr(valid), ptr(ids), ptr(weights), topk, renormalize, ptr(grad_weights), ptr(counts),
                   ptr(tokens), ptr(grad_loss), grad.data_ptr())
     return grad
 
@@ -116,7 +116,7 @@ class _Route(torch.autograd.Function):
                                                       None, balance)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(ids, counts)
-        ctx.save_for_backward(logits, valid, ids, counts if balance else None, tokens)
+        ctx.save_for_backward(logits, valid, ids, weights, counts if balance else None, tokens)
         ctx.options = topk, renormalize
         return weights, ids, counts, loss
 
@@ -125,8 +125,8 @@ class _Route(torch.autograd.Function):
         _once()
         if grad_weights is None and grad_loss is None:
             return (None,) * 5
-        logits, valid, ids, counts, tokens = ctx.saved_tensors
-        grad = _backward(logits, *ctx.options, valid, ids, grad_weights, counts, tokens,
+        logits, valid, ids, weights, counts, tokens = ctx.saved_tensors
+        grad = _backward(logits, *ctx.options, valid, ids, weights, grad_weights, counts, tokens,
                          grad_loss)
         return grad, None, None, None, None
 
@@ -147,7 +147,7 @@ class _Balance(torch.autograd.Function):
         if grad_loss is None:
             return None, None, None
         logits, valid, counts, tokens = ctx.saved_tensors
-        return _backward(logits, ctx.topk, 0, valid, None, None, counts, tokens,
+        return _backward(logits, ctx.topk, 0, valid, None, None, None, counts, tokens,
                          grad_loss), None, None
 
 
