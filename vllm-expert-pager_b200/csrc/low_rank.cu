@@ -799,6 +799,7 @@ constexpr int kLoadWarps = 4;
 constexpr int kLoaders = kLoadWarps * 32;
 constexpr int kShiftWarps = 4;               // where rows lie at any place
 constexpr int kNBlock = 64;                  // columns of out in a stage
+constexpr uint32_t kWholeBlocks = 8;         // blocks of 64 of H that are not split
 constexpr int kTmemCols = 256;               // v: 128 at most, then two blocks of out
 constexpr int kTmemOut = 128;
 constexpr int tile_threads(bool vec) {
@@ -916,7 +917,10 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
   // This CTA's blocks of 64 along H and along N.
   const uint32_t kb_all = static_cast<uint32_t>((a.H + 63) / 64);
   const uint32_t nb_all = static_cast<uint32_t>((a.N + kNBlock - 1) / kNBlock);
-  const int k0 = kb_all * rank >> log2c, k1 = kb_all * (rank + 1) >> log2c;
+  // A short H is not worth the exchange of shares (4 to 5 us): every CTA sums all of it.
+  const bool shared_v = C > 1 && kb_all > kWholeBlocks;
+  const int k0 = shared_v ? kb_all * rank >> log2c : 0;
+  const int k1 = shared_v ? kb_all * (rank + 1) >> log2c : kb_all;
   const int n0 = nb_all * rank >> log2c, n1 = nb_all * (rank + 1) >> log2c;
   const int first = k1 - k0, chunks = first + n1 - n0;
   const int k_steps = (a.r + 15) / 16;  // of the second product
@@ -1232,7 +1236,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
       for (int j = 0; j < 16; ++j) u[i][j] = 0.0f;
       if (ok && first > 0 && 2 * i + side < kRB) tc_load16(u[i], my_tmem + (2 * i + side) * 16);
     }
-    if (C > 1) {
+    if (shared_v) {
       // The cluster's shares of v, added in the order of its CTAs.  They lie where v
       // will, which is written when all have read them.
       // Four ranks of all rows together, so that a warp reads 512 bytes in a row.
@@ -1494,8 +1498,12 @@ int run_sized(LowRankArgs &a, cudaStream_t s) {
   rc = launch_status();
   if (rc) return rc;
   const int64_t tiles = most_tiles(a.M, a.slots);
-  const int64_t full = (a.M + kTile - 1) / kTile;  // tiles of a batch with few adapters
-  const int log2c = full <= 18 ? 3 : (full <= 37 ? 2 : (full <= 148 ? 1 : 0));
+  // As large a cluster for a tile as leaves all tiles on the device at once, if the
+  // adapters' last tiles are as many as the full ones or the slots.
+  const int64_t full = (a.M + kTile - 1) / kTile, guess = full + (a.slots < full ? a.slots : full);
+  const int64_t room = vec && kRB <= 4 ? 296 : 148;
+  int log2c = 3;
+  while (log2c > 0 && guess << log2c > room) --log2c;
   const void *fn = vec ? (const void *)tile_kernel<T, kRB, true>
                        : (const void *)tile_kernel<T, kRB, false>;
   const int smem = vec ? TileSmem<kRB, true>::kBytes : TileSmem<kRB, false>::kBytes;

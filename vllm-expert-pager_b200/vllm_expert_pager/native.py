@@ -98,15 +98,12 @@ XP_EINVAL = -22
 XP_ERANGE = -34
 XP_EPITCH = -75
 
-# Element types and limits of the routing and low-rank entry points.
-DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+# Limits of the routing and low-rank entry points.
 MAX_EXPERTS = 4096
-MAX_TOPK = 32
 MAX_RANK = 128
-MAX_ADAPTER_SLOTS = 8192
-MAX_TOKENS = 1 << 26
 
 _lib: ctypes.CDLL | None = None
+_ops = None
 
 
 def lib() -> ctypes.CDLL:
@@ -127,6 +124,24 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+def torch_ops():
+    """The module of the routing and low-rank operators (csrc/torch_ops.cpp, built beside
+    the library for the torch of this python)."""
+    global _ops
+    if _ops is None:
+        lib()
+        try:
+            from vllm_expert_pager import _torch_ops
+        except ImportError as e:
+            raise RuntimeError(
+                "vllm-expert-pager: the torch operators are missing or were built for another "
+                f"torch or python ({e}); build them with `make -C vllm-expert-pager_b200/csrc` "
+                "(there is no fallback path)"
+            ) from e
+        _ops = _torch_ops
+    return _ops
+
+
 def check(rc: int, what: str) -> None:
     """Raise for a non-zero status of a libxpager call."""
     if rc != XP_OK:
@@ -143,26 +158,6 @@ def ptr(t: torch.Tensor | None) -> int | None:
 def stream_of(device: torch.device) -> int:
     """Handle of the current CUDA stream of ``device`` (captured streams included)."""
     return torch.cuda.current_stream(device).cuda_stream
-
-
-def _stream(index: int) -> int:
-    return torch.cuda.current_stream(index).cuda_stream
-
-
-# The same handle without the Stream object around it (2 us less on each call).
-_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _stream)
-
-
-def launch(device: torch.device, what: str, fn, *args) -> None:
-    """Call ``fn(*args, stream)`` on the current stream of ``device``, whichever device is current."""
-    index = device.index
-    if index == torch.cuda.current_device():
-        rc = fn(*args, _stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, _stream(index))
-    if rc != XP_OK:
-        check(rc, what)
 
 
 def require_cuda(*tensors: torch.Tensor | None) -> None:
