@@ -846,6 +846,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
   __shared__ uint32_t at_x[kVec ? 1 : kTile], at_y[kVec ? 1 : kTile], at_a[kVec ? 1 : S::kR],
       at_b[kVec ? 1 : kNBlock];
   __shared__ uint16_t *out_row[kVec ? 1 : kTile];
+  __shared__ uint4 carry[kVec ? 1 : kTile];  // the last eight values of the block before
   __shared__ float amax[2][kTile];
   __shared__ uint32_t tmem_at;
   __shared__ int failed;
@@ -1369,37 +1370,44 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
                  a.N - n - piece * 8, true);
         }
       } else {
-        // Rows at any place: a row of the block for a warp, the aligned pairs of its
-        // values (the first or last value alone); both sides' columns together.
+        // Rows at any place: the aligned 16-byte words of out, each from two
+        // neighbouring pieces of a row (the first from the end of the block before);
+        // both sides' columns together.
         asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
         const int left = static_cast<int>(min(a.N - n, static_cast<int64_t>(kNBlock)));
-        const int r0 = (warp & 3) * 32 + side * 16;
-        const uint32_t here = (lane >> 2) * 16 + (lane & 3) * 4,
-                       next = (lane + 1 >> 2) * 16 + (lane + 1 & 3) * 4;
-#pragma unroll 1
-        for (int j0 = 0; j0 < 16 && ok && r0 + j0 < n_rows; j0 += 8) {
-          uint16_t *o[8];
-          uint32_t v[8], v0[8];
+        const int piece = lane & 7, r0 = (warp & 3) * 32 + side * 16 + (lane >> 3);
+        if (ok) {
+          Words w[4];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int r = r0 + j0 + j;
-            const unsigned char *row = ys + r * 128;
-            const uint32_t turn = (r & 7) << 4;
-            o[j] = out_row[r] + static_cast<int64_t>(i) * kNBlock;
-            v0[j] = *reinterpret_cast<const uint32_t *>(row + (here ^ turn));
-            v[j] = __funnelshift_r(
-                v0[j], *reinterpret_cast<const uint32_t *>(row + ((next & 127) ^ turn)),
-                (place_of(o[j]) & 2) * 8);
+          for (int j = 0; j < 4; ++j) {
+            const int r = r0 + 4 * j;
+            w[j].hi = *reinterpret_cast<const uint4 *>(ys + swizzled(r, piece));
+            w[j].lo = piece ? *reinterpret_cast<const uint4 *>(ys + swizzled(r, piece - 1 & 7))
+                            : carry[r];
           }
+          __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (r0 + j0 + j >= n_rows) break;
-            const int odd = place_of(o[j]) >> 1 & 1, pairs = (left - odd) >> 1;
-            if (lane < pairs)
-              *reinterpret_cast<uint32_t *>(o[j] + odd + 2 * lane) = v[j];
-            else if (lane == pairs && (left - odd & 1))
-              o[j][odd + 2 * lane] = static_cast<uint16_t>(v[j]);
-            if (lane == 0 && odd) o[j][0] = static_cast<uint16_t>(v0[j]);
+          for (int j = 0; j < 4; ++j) {
+            const int r = r0 + 4 * j;
+            if (r >= n_rows) break;
+            if (piece == 7) carry[r] = w[j].hi;
+            uint16_t *o = out_row[r] + static_cast<int64_t>(i) * kNBlock;
+            const int off = place_of(o), e0 = piece * 8 - off / 2;  // the word's first value
+            const uint4 q = off ? join_words(w[j], 16 - off, 8) : w[j].hi;
+            if ((e0 >= 0 || i > 0) && e0 + 8 <= left) {
+              *reinterpret_cast<uint4 *>(o + e0) = q;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if ((e0 + e >= 0 || i > 0) && e0 + e < left)
+                  o[e0 + e] = static_cast<uint16_t>((&q.x)[e >> 1] >> (16 * (e & 1)));
+            }
+            if (piece == 7 && c == chunks - 1) {  // what is left behind the last word
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (56 + e >= e0 + 8 && 56 + e < left)
+                  o[56 + e] = static_cast<uint16_t>((&w[j].hi.x)[e >> 1] >> (16 * (e & 1)));
+            }
           }
         }
         asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
