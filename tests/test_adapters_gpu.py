@@ -194,6 +194,31 @@ def test_what_no_row_uses_is_not_read(M):
     assert torch.equal(keep.isnan(), o["x"].isnan())
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M", [3, 70, 1500])
+def test_aligned_rows_that_end_inside_a_vector(dtype, M):
+    """Rows on 16-byte boundaries whose widths are no multiple of 8: the values behind a row's
+    end are neither used nor written."""
+    S = 5
+    for H, N, r in ((192, 131, 24), (512, 1999, 64), (189, 136, 16), (77, 65, 5)):
+        o, g = make(M, H, N, r, S, dtype, seed=M + N)
+        slots = torch.randint(-1, S, (M,), generator=g, device=DEV)
+        pitch = (max(H, N) + 23) // 8 * 8
+        wide = {k: torch.full((M, pitch), math.nan, dtype=dtype, device=DEV)
+                for k in ("x", "y", "out")}
+        x, y, out = wide["x"][:, :H], wide["y"][:, 8 : 8 + N], wide["out"][:, :N]
+        x.copy_(o["x"])
+        y.copy_(o["y"])
+        check({**o, "x": x, "y": y}, slots, slots, out=out)
+        assert wide["out"][:, N:].isnan().all()
+        want = wide["out"][:, :N].clone()
+        from vllm_expert_pager import adapters
+
+        adapters.add_low_rank(y, x, o["a"], o["b"], slots, scale=o["scale"])  # in place
+        assert torch.equal(y, want)
+        assert wide["y"][:, :8].isnan().all() and wide["y"][:, 8 + N :].isnan().all()
+
+
 @pytest.mark.parametrize("M", [2, 40, 1200])
 def test_rows_are_apart(M):
     """A row's result is the same bits whatever rows it shares the batch with, in any order."""

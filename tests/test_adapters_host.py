@@ -110,6 +110,9 @@ def test_overlap_is_refused():
     buf = torch.zeros((7, 24), dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="overlap"):  # out one row behind y
         adapters.add_low_rank(**{**o, "y": buf[:6], "out": buf[1:]})
+    slab = torch.zeros((3 * 24 * 4,), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="overlap the adapter slabs"):
+        adapters.add_low_rank(**{**o, "b": slab.view(3, 24, 4), "out": slab[:144].view(6, 24)})
     wide = torch.zeros((6, 40), dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="overlap"):  # columns of out run into x's
         adapters.add_low_rank(**{**o, "x": wide[:, :24], "out": wide[:, 16:]})

@@ -323,6 +323,9 @@ Tensor add_low_rank(const Tensor &y_in, const Tensor &x_in, const Tensor &a, con
     require(!overlap(at(out), out.stride(0), N, at(x), x.stride(0), H, M) &&
                 (same || !overlap(at(out), out.stride(0), N, at(y), y.stride(0), N, M)),
             "out may be y itself, and may not overlap x or other rows of y");
+    for (const Tensor *v : {&a, &b})
+      require(at(*v) + 2 * v->numel() <= at(out) || at(out) + 2 * ((M - 1) * out.stride(0) + N) <= at(*v),
+              "out may not overlap the adapter slabs");
   }
   for (const Tensor *v : {&x_in, &y_in, &a, &b, &ids_in, &out}) require_cuda(*v);
   if (scale_in) require_cuda(*scale_in);
