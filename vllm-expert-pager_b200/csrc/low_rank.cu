@@ -1526,11 +1526,14 @@ int run_sized(LowRankArgs &a, cudaStream_t s) {
   if (rc) return rc;
   const int64_t tiles = most_tiles(a.M, a.slots);
   // As large a cluster for a tile as leaves all tiles on the device at once, if half
-  // of the slots are in use (the host does not know): 1536 rows of 256 adapters in
-  // 256 slots take 139 us in clusters of 8, of 4 adapters 19 us there.
+  // of the slots are in use (the host does not know): 1536 rows of 256 adapters in 256
+  // slots take 63 us in clusters of 2 and 139 us of 8, of 4 adapters 30 and 19 us.
   const int64_t full = (a.M + kTile - 1) / kTile, guess = full + a.slots / 2;
   const int64_t room = vec && kRB <= 4 ? 296 : 148;
-  int log2c = 3;
+  // Where shares of v are exchanged, four CTAs at most: 4096 rows, 2048 -> 2048 (us, clusters of
+  // 1 / 2 / 4 / 8): rank 16 48 / 32 / 24 / 27, rank 64 53 / 35 / 28 / 48; 2048 rows, rank 32
+  // 48 / 31 / 23 / 29.
+  int log2c = a.H > 64 * static_cast<int64_t>(kWholeBlocks) ? 2 : 3;
   while (log2c > 0 && guess << log2c > room) --log2c;
   const void *fn = vec ? (const void *)tile_kernel<T, kRB, true>
                        : (const void *)tile_kernel<T, kRB, false>;
