@@ -286,7 +286,7 @@ __device__ __forceinline__ float row_max(const float *v, bool *live) {
 }
 
 struct ForwardArgs {
-  const void *logits;  // NULL: counts of given ids only
+  const void *logits;
   int64_t T, stride;
   int E, topk, renormalize;
   const uint8_t *valid;
@@ -404,10 +404,8 @@ __global__ void __launch_bounds__(forward_threads(VPL), forward_blocks(VPL))
         }
       }
     }
-    if (!kAhead) {
-      // (Two rows do not fit the registers; the values are read again below.)
-      next_live = counts(t + 2 * step);
-    }
+    // Where two rows do not fit the registers the next one is fetched at the end.
+    if (!kAhead) next_live = counts(t + 2 * step);
     if constexpr (kGiven) {
       for (int j = lane; j < a.topk; j += 32) {
         if (j >= 32) given = load_id(a.given, a.given_bytes, t * a.topk + j);
