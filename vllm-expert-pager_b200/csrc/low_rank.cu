@@ -24,9 +24,9 @@
 //    B and y, through one ring of shared-memory stages, one thread issues tcgen05
 //    instructions with the sums in tensor memory, and eight warps make v's parts
 //    and write out.  The second product's operands are on their way while the
-//    first one ends.  B200, 16384 rows, rank 64, 2048 -> 2048: 54 us, both products
-//    at 6 to 7 TB/s, 4 us between them.  (mma.sync on 64-row tiles took 87: its
-//    instructions alone fill the tensor pipe for 29 us at that rank.)
+//    first one ends.  B200, 16384 rows, rank 64, 2048 -> 2048: 53 us against 32 of
+//    HBM; a tile's chain of 64 blocks alone takes 45.  (mma.sync on 64-row tiles took
+//    87: its instructions alone fill the tensor pipe for 29 us at that rank.)
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -818,16 +818,17 @@ constexpr int kNBlock = 64;                  // columns of out in a stage
 constexpr uint32_t kWholeBlocks = 12;
 constexpr int kTmemCols = 256;               // v: 128 at most, then two blocks of out
 constexpr int kTmemOut = 128;
+constexpr int kWholeSm = 208 * 1024;         // shared memory that leaves no room for another CTA
 constexpr int tile_threads(bool vec) {
   return (kOutWarps + 1 + kLoadWarps + (vec ? 0 : kShiftWarps)) * 32;
 }
 
 // kRB: blocks of 16 ranks.  kAtoms: 128-byte rows that hold a row of ranks.
-template <int kRB, bool kVec>
+template <int kRB, bool kVec, bool kDeep>
 struct TileSmem {
   static constexpr int kR = kRB * 16;
   static constexpr int kAtoms = kR > 64 ? 2 : 1;
-  static constexpr int kStages = kVec || kRB <= 4 ? 3 : 2;
+  static constexpr int kStages = kDeep ? (kRB <= 4 ? 6 : 4) : (kVec || kRB <= 4 ? 3 : 2);
   // A stage holds 128 rows x 64 values of x and kR x 64 of A, or 64 rows of B and 128 x 64 of y.
   static constexpr int kA = kTile * 128;
   static constexpr int kY = kAtoms * kNBlock * 128;
@@ -847,11 +848,11 @@ struct TileSmem {
 };
 
 // kVec: all rows allow 16-byte accesses; else four more warps shift what the loading
-// warps bring.
-template <typename T, int kRB, bool kVec>
-__global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
+// warps bring.  kDeep: twice the stages, one CTA on an SM.
+template <typename T, int kRB, bool kVec, bool kDeep>
+__global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep ? 2 : 1)
     tile_kernel(const __grid_constant__ LowRankArgs a) {
-  using S = TileSmem<kRB, kVec>;
+  using S = TileSmem<kRB, kVec, kDeep>;
   constexpr int kStages = S::kStages;
   const bool vec_y = kVec || a.vec_y;
   extern __shared__ unsigned char raw[];
@@ -922,7 +923,10 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     tc_fence_before();
   }
-  if (C > 1)
+  // A short H is not worth the exchange of shares: every CTA sums all of it.
+  const uint32_t kb_all = static_cast<uint32_t>((a.H + 63) / 64);
+  const bool shared_v = C > 1 && kb_all > kWholeBlocks;
+  if (shared_v)
     cluster.sync();
   else
     __syncthreads();
@@ -932,10 +936,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
   const T *A = static_cast<const T *>(a.a) + static_cast<int64_t>(s) * a.r * a.H;
   const T *B = static_cast<const T *>(a.b) + static_cast<int64_t>(s) * a.r * a.N;
   // This CTA's blocks of 64 along H and along N.
-  const uint32_t kb_all = static_cast<uint32_t>((a.H + 63) / 64);
   const uint32_t nb_all = static_cast<uint32_t>((a.N + kNBlock - 1) / kNBlock);
-  // A short H is not worth the exchange of shares: every CTA sums all of it.
-  const bool shared_v = C > 1 && kb_all > kWholeBlocks;
   const int k0 = shared_v ? kb_all * rank >> log2c : 0;
   const int k1 = shared_v ? kb_all * (rank + 1) >> log2c : kb_all;
   const int n0 = nb_all * rank >> log2c, n1 = nb_all * (rank + 1) >> log2c;
@@ -1433,7 +1434,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 ? 2 : 1)
     }
   }
   tc_fence_before();
-  if (C > 1)
+  if (shared_v)
     cluster.sync();  // a CTA's barriers stay until the cluster has used them
   else
     __syncthreads();
@@ -1525,19 +1526,33 @@ int run_sized(LowRankArgs &a, cudaStream_t s) {
   rc = launch_status();
   if (rc) return rc;
   const int64_t tiles = most_tiles(a.M, a.slots);
+  // Where shares of v are exchanged, CTAs wait for one another while they hold tensor
+  // memory.  With two CTAs on an SM, or another kernel's beside one, such clusters
+  // could each hold what the other's next CTA waits for; so these launches take an
+  // SM's shared memory whole, and nothing that uses tensor memory fits beside them.
+  const bool shares = a.H > 64 * static_cast<int64_t>(kWholeBlocks);
   // As large a cluster for a tile as leaves all tiles on the device at once, if half
-  // of the slots are in use (the host does not know): 1536 rows of 256 adapters in 256
-  // slots take 63 us in clusters of 2 and 139 us of 8, of 4 adapters 30 and 19 us.
+  // of the slots are in use (the host does not know).  Measured at 2048 -> 2048, 6 adapters
+  // in 8 slots (us, clusters of 1 / 2 / 4): rank 16, 3000 rows 44 / 29 / 22, 4096 45 / 30 / 37
+  // (more tiles than fit), 8192 45 / 31 / 40, 12000 46 / 57 / 57; rank 64, 8192 49 / 34 / 48.
+  // At 512 -> 2048, nothing exchanged and two CTAs on an SM, 2048 rows take 18 in clusters of 8.
   const int64_t full = (a.M + kTile - 1) / kTile, guess = full + a.slots / 2;
-  const int64_t room = vec && kRB <= 4 ? 296 : 148;
-  // Where shares of v are exchanged, four CTAs at most: 4096 rows, 2048 -> 2048 (us, clusters of
-  // 1 / 2 / 4 / 8): rank 16 48 / 32 / 24 / 27, rank 64 53 / 35 / 28 / 48; 2048 rows, rank 32
-  // 48 / 31 / 23 / 29.
-  int log2c = a.H > 64 * static_cast<int64_t>(kWholeBlocks) ? 2 : 3;
-  while (log2c > 0 && guess << log2c > room) --log2c;
-  const void *fn = vec ? (const void *)tile_kernel<T, kRB, true>
-                       : (const void *)tile_kernel<T, kRB, false>;
-  const int smem = vec ? TileSmem<kRB, true>::kBytes : TileSmem<kRB, false>::kBytes;
+  const bool two = vec && kRB <= 4;  // two CTAs fit on an SM
+  int log2c = 0;
+  if (shares)
+    log2c = guess * 4 <= 132 ? 2 : (guess * 2 <= 144 ? 1 : 0);
+  else
+    for (log2c = 3; log2c > 0 && guess << log2c > (two ? 296 : 148);) --log2c;
+  // One CTA on an SM with a deep ring up to as many tiles as SMs, then two (16384 rows, rank
+  // 64, 2048 -> 2048: 52 / 62 us; 24000 rows: 96 / 84).
+  const bool deep = vec && (!two || (shares && guess << log2c <= 148));
+  const void *fn = deep ? (const void *)tile_kernel<T, kRB, true, true>
+                        : (vec ? (const void *)tile_kernel<T, kRB, true, kRB == 8>
+                               : (const void *)tile_kernel<T, kRB, false, false>);
+  int smem = deep ? TileSmem<kRB, true, true>::kBytes
+                  : (vec ? TileSmem<kRB, true, kRB == 8>::kBytes
+                         : TileSmem<kRB, false, false>::kBytes);
+  if (shares && log2c > 0 && smem < kWholeSm) smem = kWholeSm;
   return launch(fn, tiles, log2c, tile_threads(vec), smem, nullptr, true, a, s);
 }
 
