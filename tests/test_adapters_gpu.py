@@ -453,3 +453,29 @@ def test_pager_refusals():
     finally:
         pager.release()
         pager.release()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M, H, N, r", [
+    (1, 2048, 1024, 16), (5, 3, 7, 2), (40, 200, 40, 33), (300, 1021, 131, 128),
+    (1100, 512, 72, 16), (1100, 835, 65, 40), (2000, 1024, 128, 64), (1500, 96, 31, 100),
+    (3000, 512, 256, 64), (9000, 1024, 192, 48), (20000, 832, 128, 64), (20000, 832, 64, 128)])
+def test_low_rank_values_are_whole(dtype, M, H, N, r):
+    """Two low-rank values that agree in all but their last bits, subtracted: what is left is
+    exact only if they enter the second product with the 24 bits of their sums."""
+    from vllm_expert_pager import adapters
+
+    S = 3
+    most, least = {torch.bfloat16: (2.0 ** -9, 2.0 ** -19),
+                   torch.float16: (2.0 ** -12, 2.0 ** -23)}[dtype]
+    x = torch.zeros((M, H), dtype=dtype, device=DEV)
+    a = torch.zeros((S, r, H), dtype=dtype, device=DEV)
+    b = torch.zeros((S, N, r), dtype=dtype, device=DEV)
+    at = [0, H // 2, H - 1]
+    x[:, at] = 1.0
+    a[:, 0, at] = torch.tensor([1.0, most, least], dtype=dtype, device=DEV)
+    a[:, r - 1, at] = torch.tensor([1.0, most, 0.0], dtype=dtype, device=DEV)
+    b[:, :, 0], b[:, :, r - 1] = 1.0, -1.0
+    ids = torch.arange(M, dtype=torch.int32, device=DEV) % S
+    got = adapters.add_low_rank(torch.zeros((M, N), dtype=dtype, device=DEV), x, a, b, ids)
+    assert torch.equal(got, torch.full_like(got, least))

@@ -2,9 +2,9 @@
 // s of every row from its adapter id.
 //
 // Both products run on the tensor cores (16-bit operands, 32-bit sums).  Between
-// them stands v = scale_s x A_s^T, r values a row, kept as two 16-bit parts
-// (v = hi + lo): the second product then loses 2^-16 of v at most, where one part
-// would lose as much as the output's own rounding.  float16 parts are taken of v
+// them stands v = scale_s x A_s^T, r values a row, which enters the second product
+// whole, as the sum of three 16-bit parts (8 or 11 bits each; two of bfloat16 would
+// lose 2^-16 of v, which shows where v's terms cancel).  float16 parts are taken of v
 // times the power of two that brings the row's largest magnitude to 2^14, so that
 // neither end of the type's range is left.
 //
@@ -85,6 +85,11 @@ struct Half<__nv_bfloat16> {
     __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t *>(&h);
   }
+  static __device__ __forceinline__ uint32_t cut(float lo, float hi) {
+    uint32_t w;
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    return w;
+  }
   static __device__ __forceinline__ float2 unpack(uint32_t w) {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }
@@ -104,6 +109,11 @@ struct Half<__half> {
     __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<uint32_t *>(&h);
   }
+  static __device__ __forceinline__ uint32_t cut(float lo, float hi) {
+    uint32_t w;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    return w;
+  }
   static __device__ __forceinline__ float2 unpack(uint32_t w) {
     return __half22float2(*reinterpret_cast<__half2 *>(&w));
   }
@@ -122,20 +132,23 @@ __device__ __forceinline__ float widen(__half x) { return __half2float(x); }
 __device__ __forceinline__ void narrow(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 __device__ __forceinline__ void narrow(__half *p, float x) { *p = __float2half_rn(x); }
 
-// The high and the low part of two neighbouring values.  Where the high part is
-// not finite the low part is 0, so that an infinity stays one.
+// The parts of two neighbouring values, cut and not rounded, so that each is exact and
+// none leaves the range.  Of what is not finite the first part holds all.
 template <typename T>
-__device__ __forceinline__ void split(float u, float w, uint32_t *hi, uint32_t *lo) {
-  *hi = Half<T>::pack(u, w);
-  const float2 h = Half<T>::unpack(*hi);
-  *lo = Half<T>::pack(isfinite(h.x) ? u - h.x : 0.0f, isfinite(h.y) ? w - h.y : 0.0f);
+__device__ __forceinline__ void split(float u, float w, uint32_t (&part)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    part[i] = Half<T>::cut(u, w);
+    const float2 h = Half<T>::unpack(part[i]);
+    u = isfinite(h.x) ? u - h.x : 0.0f, w = isfinite(h.y) ? w - h.y : 0.0f;
+  }
 }
 
 // The power of two that brings a row's largest magnitude into [2^14, 2^15); 1 for
 // rows of zeros (or less than 2^-126), of infinities and of NaN.
 __device__ __forceinline__ float range_factor(float amax) {
   const int e = static_cast<int>(__float_as_uint(amax) >> 23);  // the biased exponent
-  return e == 0 || e >= 254 ? 1.0f
+  return e == 0 || e == 255 ? 1.0f
                             : __uint_as_float(static_cast<uint32_t>(min(268 - e, 253)) << 23);
 }
 
@@ -292,10 +305,10 @@ __global__ void __launch_bounds__(kThreads, kVec && kRB <= 4 ? 3 : 2)
   extern __shared__ __align__(128) unsigned char smem[];
   constexpr int kPitchV = kR + 4;
   // The warps' sums of v; when they have been added up, v's parts.
-  constexpr int kRed = kParts * kGroup * kPitchV * 4, kParts2 = 2 * kGroup * (kR + 8) * 2;
-  __shared__ __align__(16) unsigned char room[kRed > kParts2 ? kRed : kParts2];
+  constexpr int kRed = kParts * kGroup * kPitchV * 4, kSplit = 3 * kGroup * (kR + 8) * 2;
+  __shared__ __align__(16) unsigned char room[kRed > kSplit ? kRed : kSplit];
   float(*red)[kGroup * kPitchV] = reinterpret_cast<float(*)[kGroup * kPitchV]>(room);
-  uint16_t(*vhi)[kR + 8] = reinterpret_cast<uint16_t(*)[kR + 8]>(room), (*vlo)[kR + 8] = vhi + kGroup;
+  uint16_t(*vs)[kGroup][kR + 8] = reinterpret_cast<uint16_t(*)[kGroup][kR + 8]>(room);
   __shared__ __align__(8) float part[kGroup * kPitchV];  // [row][rank]: this CTA's share of v
   __shared__ float factor[kGroup];
   static_assert(XP_MAX_ADAPTER_SLOTS <= INT16_MAX, "slots fit 16 bits");
@@ -532,22 +545,23 @@ __global__ void __launch_bounds__(kThreads, kVec && kRB <= 4 ? 3 : 2)
 #pragma unroll
       for (int i = 0; i < kEach; ++i)
         if (i * 64 + 2 * lane < kR) {
-          uint32_t hi, lo;
-          split<T>(u[i][0] * f, u[i][1] * f, &hi, &lo);
-          *reinterpret_cast<uint32_t *>(&vhi[warp][i * 64 + 2 * lane]) = hi;
-          *reinterpret_cast<uint32_t *>(&vlo[warp][i * 64 + 2 * lane]) = lo;
+          uint32_t q[3];
+          split<T>(u[i][0] * f, u[i][1] * f, q);
+#pragma unroll
+          for (int p = 0; p < 3; ++p)
+            *reinterpret_cast<uint32_t *>(&vs[p][warp][i * 64 + 2 * lane]) = q[p];
         }
       if (lane == 0) factor[warp] = 1.0f / f;
     }
     __syncthreads();
 
     // out^T[n, row]: B as the 16 rows of an instruction, v's parts as its 8 columns.
-    uint32_t hi[kRB][2], lo[kRB][2];
+    uint32_t v[kRB][3][2];
 #pragma unroll
-    for (int i = 0; i < kRB; ++i) {
-      ldmatrix2(hi[i], smem_addr(&vhi[lane & 7][i * 16 + ((lane >> 3) & 1) * 8]));
-      ldmatrix2(lo[i], smem_addr(&vlo[lane & 7][i * 16 + ((lane >> 3) & 1) * 8]));
-    }
+    for (int i = 0; i < kRB; ++i)
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+        ldmatrix2(v[i][p], smem_addr(&vs[p][lane & 7][i * 16 + ((lane >> 3) & 1) * 8]));
     const float f0 = factor[2 * t], f1 = factor[2 * t + 1];
 #pragma unroll 1
     for (int c = first; c < chunks; ++c) {
@@ -564,8 +578,9 @@ __global__ void __launch_bounds__(kThreads, kVec && kRB <= 4 ? 3 : 2)
         for (int i = 0; i < kRB; ++i) {
           uint32_t p[4];
           ldmatrix4(p, at + (b + (lane & 15)) * S::kPitchB + i * 32 + (lane >> 4) * 16);
-          Half<T>::mma(d, p[0], p[1], p[2], p[3], hi[i][0], hi[i][1]);
-          Half<T>::mma(d, p[0], p[1], p[2], p[3], lo[i][0], lo[i][1]);
+#pragma unroll
+          for (int q = 0; q < 3; ++q)
+            Half<T>::mma(d, p[0], p[1], p[2], p[3], v[i][q][0], v[i][q][1]);
         }
         // y + update in place of y in the stage, then 16-byte pieces of out.
 #pragma unroll
@@ -776,13 +791,32 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr) {
          (1ull << 46) | (2ull << 61);
 }
 
-// d[128, N] (+)= a[128, 16] b[N, 16]^T, 32-bit sums in tensor memory.
+// d[128, N] (+)= a[128, 16] b[N, 16]^T, 32-bit sums in tensor memory, both operands in
+// shared memory.
 __device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t what,
                                        bool add) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(what), "r"(static_cast<uint32_t>(add))
+      : "memory");
+}
+
+// The same with a in tensor memory: a lane for each row, two neighbouring values a column.
+__device__ __forceinline__ void tc_mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t what,
+                                            bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(what), "r"(static_cast<uint32_t>(add))
+      : "memory");
+}
+
+// Eight columns of this thread's row of tensor memory.
+__device__ __forceinline__ void tc_store8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
       : "memory");
 }
 
@@ -816,8 +850,12 @@ constexpr int kNBlock = 64;                  // columns of out in a stage
 // whole / split): H 256 16.5 / 21.8, 512 17.8 / 21.3, 768 19.3 / 21.7, 1024 21.2 / 21.8,
 // 2048 27.2 / 22.7; with 4096 rows 768 21.6 / 21.2.
 constexpr uint32_t kWholeBlocks = 12;
-constexpr int kTmemCols = 256;               // v: 128 at most, then two blocks of out
-constexpr int kTmemOut = 128;
+// Tensor memory: v's sums, and when they have been read two blocks of out in their place;
+// behind them v's parts, two values a column.  All parts are there, none in shared memory:
+// an instruction with an operand from tensor memory does not wait for one before it that
+// takes both from shared memory, on the same sum (the product of the last of those was lost).
+constexpr int kTmemV = 128;
+constexpr int tmem_cols(int blocks) { return blocks <= 4 ? 256 : 512; }
 constexpr int kWholeSm = 208 * 1024;         // shared memory that leaves no room for another CTA
 constexpr int tile_threads(bool vec) {
   return (kOutWarps + 1 + kLoadWarps + (vec ? 0 : kShiftWarps)) * 32;
@@ -834,9 +872,7 @@ struct TileSmem {
   static constexpr int kY = kAtoms * kNBlock * 128;
   static constexpr int kFirst = kA + kR * 128, kSecond = kY + kTile * 128;
   static constexpr int kStage = ((kFirst > kSecond ? kFirst : kSecond) + 1023) / 1024 * 1024;
-  // The high parts of v, then the low parts; before them this CTA's share of v (32-bit).
-  static constexpr int kV = 2 * kAtoms * kTile * 128;
-  static_assert(kR * kTile * 4 <= kV, "a share of v has room where v goes");
+  static constexpr int kShare = kR * kTile * 4;  // this CTA's share of v
   // Rows at any place come as the aligned 16-byte words around them, one more than
   // the stage's row has; shifting them fills the stage.
   static constexpr int kWords = kVec ? 0 : (kRB <= 4 ? 4 : 2);  // such stages
@@ -844,7 +880,7 @@ struct TileSmem {
   static constexpr int kWordsA = kTile * kPitch, kWordsY = kNBlock * kPitchB;
   static constexpr int kWords1 = kWordsA + kR * kPitch, kWords2 = kWordsY + kTile * kPitch;
   static constexpr int kWordsStage = kWords1 > kWords2 ? kWords1 : kWords2;
-  static constexpr int kBytes = 1024 + kStages * kStage + kV + kWords * kWordsStage;
+  static constexpr int kBytes = 1024 + kStages * kStage + kShare + kWords * kWordsStage;
 };
 
 // kVec: all rows allow 16-byte accesses; else four more warps shift what the loading
@@ -857,7 +893,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
   const bool vec_y = kVec || a.vec_y;
   extern __shared__ unsigned char raw[];
   __shared__ int64_t rows[kTile];
-  __shared__ __align__(8) uint64_t bars[3 * kStages + 8 + 2 * S::kWords];
+  __shared__ __align__(8) uint64_t bars[3 * kStages + 7 + 2 * S::kWords];
   // Not kVec: where a row's first value lies in its words (bytes), and in the upper
   // half the bits to shift by; the rows' first values of out in this CTA's part.
   __shared__ uint32_t at_x[kVec ? 1 : kTile], at_y[kVec ? 1 : kTile], at_a[kVec ? 1 : S::kR],
@@ -878,14 +914,14 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
   const int s = job.x, n_rows = job.z;
   unsigned char *smem =
       raw + ((1024 - (static_cast<uint32_t>(__cvta_generic_to_shared(raw)) & 1023)) & 1023);
-  const uint32_t ring = smem_addr(smem), v_at = ring + kStages * S::kStage;
+  const uint32_t ring = smem_addr(smem);
   // Stage filled; stage free after the first / the second product; v in tensor
-  // memory; v in shared memory; a block of out in tensor memory, and read from it;
-  // the cluster's shares of v written, and read; words arrived, and shifted.
+  // memory; v's parts there; a block of out there, and read from it; the cluster's
+  // shares of v written; words arrived, and shifted.
   const uint32_t full = smem_addr(bars), free1 = full + 8 * kStages, free2 = free1 + 8 * kStages;
   const uint32_t v_done = free2 + 8 * kStages, v_ready = v_done + 8, out_done = v_ready + 8,
-                 out_read = out_done + 16, shares = out_read + 16, shares_read = shares + 8,
-                 words_full = shares_read + 8, words_free = words_full + 8 * S::kWords;
+                 out_read = out_done + 16, shares = out_read + 16, words_full = shares + 8,
+                 words_free = words_full + 8 * S::kWords;
   volatile int *fail = &failed;
 
   if (tid < kTile) rows[tid] = a.perm[job.y + min(tid, n_rows - 1)];
@@ -908,7 +944,6 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
       bar_init(out_read + 8 * i, kOutWarps * 32);
     }
     bar_init(shares, C);
-    bar_init(shares_read, C);
     for (int i = 0; i < S::kWords; ++i) {
       bar_init(words_full + 8 * i, kLoaders);
       bar_init(words_free + 8 * i, kLoaders);
@@ -918,7 +953,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_addr(&tmem_at)),
-                 "n"(kTmemCols)
+                 "n"(tmem_cols(kRB))
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     tc_fence_before();
@@ -1050,7 +1085,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
     } else if (warp <= kMmaWarp + kLoadWarps) {
       // Words: the eight of a thread's rows that begin at its piece, and the ninth of
       // one row.  A word is read where it holds a value of the row.
-      const uint32_t words = v_at + S::kV;
+      const uint32_t words = ring + kStages * S::kStage + S::kShare;
       auto begin_words = [&](int c) {
         const int stage = c % S::kWords, use = c / S::kWords;
         if (use > 0 && !bar_wait(words_free + 8 * stage, (use - 1) & 1, fail)) return 0u;
@@ -1125,7 +1160,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
     } else {
       // Shifting, from the words to a stage: two values a lane, a row of 64 for a warp
       // (whole rows of shared memory, no two lanes at one bank).
-      const unsigned char *words = smem + kStages * S::kStage + S::kV;
+      const unsigned char *words = smem + kStages * S::kStage + S::kShare;
       const int sw = p >> 5;
       // Values 2 i and 2 i + 1 of the row at `place` (see above).
       auto two = [](const unsigned char *src, uint32_t place, int i) {
@@ -1228,12 +1263,19 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
         if (!ok) break;
         fence_async_proxy();
         tc_fence_after();
-        const uint32_t at = ring + stage * S::kStage, d = tmem + kTmemOut + half * kNBlock;
-        for (int part = 0; part < 2; ++part)
-          for (int j = 0; j < k_steps; ++j)
-            tc_mma(d,
-                   operand(v_at + (part * S::kAtoms + j / 4) * kTile * 128 + 32 * (j % 4)),
-                   operand(at + (j / 4) * kNBlock * 128 + 32 * (j % 4)), kWhat2, part + j > 0);
+        const uint32_t at = ring + stage * S::kStage, d = tmem + half * kNBlock;
+        // A lone thread issues these: places are constants added to one descriptor (with
+        // each computed anew 16384 rows of rank 64 took 60 us, not 52).
+        const uint64_t b_at = operand(at);
+#pragma unroll
+        for (int part = 0; part < 3; ++part)
+#pragma unroll
+          for (int j = 0; j < kRB; ++j) {
+            if (j >= k_steps) break;
+            tc_mma_tmem(d, tmem + kTmemV + (part * kRB + j) * 8,
+                        b_at + ((j / 4) * kNBlock * 128 + 32 * (j % 4)) / 16, kWhat2,
+                        part + j > 0);
+          }
         tc_commit(out_done + 8 * half);
       }
     }
@@ -1255,9 +1297,8 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
       if (ok && first > 0 && 2 * i + side < kRB) tc_load16(u[i], my_tmem + (2 * i + side) * 16);
     }
     if (shared_v) {
-      // The cluster's shares of v, added in the order of its CTAs.  They lie where v
-      // will, which is written when all have read them.
-      // Four ranks of all rows together, so that a warp reads 512 bytes in a row.
+      // The cluster's shares of v, added in the order of its CTAs.  Four ranks of all
+      // rows together, so that a warp reads 512 bytes in a row.
       float4 *share = reinterpret_cast<float4 *>(smem + kStages * S::kStage) + row;
 #pragma unroll
       for (int i = 0; i < kMine; ++i)
@@ -1299,9 +1340,6 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
             }
           }
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (ok && tid < C) bar_arrive_peer(shares_read, tid);
-      ok = __all_sync(kFull, ok && bar_wait<true>(shares_read, 0, fail));
     }
     float f = 1.0f;
 #pragma unroll
@@ -1323,19 +1361,18 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
         if (2 * i + side >= kRB) continue;
+        uint32_t q[3][8];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            split<T>(u[i][h * 8 + 2 * j] * f, u[i][h * 8 + 2 * j + 1] * f, &hi[j], &lo[j]);
-          const int e = 2 * (2 * i + side) + h;  // 16-byte piece of the row
-          const uint32_t at = v_at + (e / 8) * kTile * 128 + swizzled(row, e % 8);
-          store16(at, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-          store16(at + S::kAtoms * kTile * 128, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+        for (int j = 0; j < 8; ++j) {
+          uint32_t w[3];
+          split<T>(u[i][2 * j] * f, u[i][2 * j + 1] * f, w);
+          q[0][j] = w[0], q[1][j] = w[1], q[2][j] = w[2];
         }
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+          tc_store8(my_tmem + kTmemV + (p * kRB + 2 * i + side) * 8, q[p]);
       }
-      fence_async_proxy();
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       tc_fence_before();
       bar_arrive(v_ready);
     }
@@ -1356,7 +1393,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
         for (int h = 0; h < 2; ++h)
           q[h] = *reinterpret_cast<const uint4 *>(ys + swizzled(row, 2 * j + h));
         float d[16];
-        tc_load16(d, my_tmem + kTmemOut + half * kNBlock + j * 16);
+        tc_load16(d, my_tmem + half * kNBlock + j * 16);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -1435,13 +1472,13 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
   }
   tc_fence_before();
   if (shared_v)
-    cluster.sync();  // a CTA's barriers stay until the cluster has used them
+    cluster.sync();  // a CTA's barriers and its share stay until the cluster has used them
   else
     __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                 "n"(kTmemCols));
+                 "n"(tmem_cols(kRB)));
   }
   if (failed) {  // a wait gave up: the rows must not pass for results
     for (int i = 0; i < n_rows; ++i)
