@@ -479,3 +479,90 @@ def test_low_rank_values_are_whole(dtype, M, H, N, r):
     ids = torch.arange(M, dtype=torch.int32, device=DEV) % S
     got = adapters.add_low_rank(torch.zeros((M, N), dtype=dtype, device=DEV), x, a, b, ids)
     assert torch.equal(got, torch.full_like(got, least))
+
+
+def classes(t):
+    """Of every value: 0 finite, 1 and -1 the infinities, 2 NaN."""
+    return torch.where(t.isnan(), 2, torch.where(t.isinf(), t.sign(), 0.0)).to(torch.int8)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M, H, N", [(6, 64, 40), (50, 61, 37), (1100, 64, 72), (1100, 835, 65),
+                                     (1100, 1024, 128)])
+@pytest.mark.parametrize("r", [1, 2, 8, 13, 16, 24, 65, 128])
+def test_infinities_are_those_of_the_definition(dtype, M, H, N, r):
+    """Infinite values of x, a and b give the infinity or the NaN that the sums of the
+    definition give, in the rows and columns that they reach, and nothing elsewhere."""
+    from vllm_expert_pager import adapters
+
+    S = 2
+    o, g = make(M, H, N, r, S, dtype, seed=M + r)
+    slots = torch.arange(M, device=DEV) % S
+
+    def run():
+        return adapters.add_low_rank(o["y"], o["x"], o["a"], o["b"], slots, scale=o["scale"],
+                                     out=fresh(o))
+
+    def want():
+        out = o["y"].double()
+        for s in range(S):
+            m = slots == s
+            v = (o["x"][m].double()[:, None, :] * o["a"][s].double()).sum(2)
+            out[m] += o["scale"][s].double() * (v[:, None, :] * o["b"][s].double()).sum(2)
+        return out
+
+    for positive in (False, True):
+        if positive:
+            o = {k: t.abs() for k, t in o.items()}
+        clean = run()
+        o["x"][2, 5] = math.inf
+        o["x"][3, 7] = -math.inf
+        keep = o["b"][1, 11 % N].clone()
+        o["b"][1, 11 % N, r // 2] = -math.inf
+        got, ref = run(), want()
+        assert torch.equal(classes(got), classes(ref.to(dtype)))
+        same = torch.ones_like(got, dtype=torch.bool)
+        same[2], same[3] = False, False
+        same[slots == 1, 11 % N] = False
+        assert torch.equal(got[same], clean[same])
+        if positive:  # sums of one sign: nothing cancels
+            assert (got[2] == math.inf).sum() == N and (got[3] == -math.inf).sum() >= N - 1
+        o["x"][2, 5] = o["x"][3, 7] = 1.0
+        o["b"][1, 11 % N] = keep
+
+
+@pytest.mark.parametrize("M", [4, 1100])
+def test_values_beside_an_infinity_and_at_the_range_end(M):
+    """An infinite low-rank value beside a finite one beyond float16's range, which b gives the
+    other sign; and in bfloat16 a finite one above bfloat16's largest."""
+    from vllm_expert_pager import adapters
+
+    H, N = 16, 24
+    ids = torch.zeros((M,), dtype=torch.int32, device=DEV)
+
+    def zeros(dtype, r):
+        return (torch.zeros((M, N), dtype=dtype, device=DEV),
+                torch.zeros((M, H), dtype=dtype, device=DEV),
+                torch.zeros((1, r, H), dtype=dtype, device=DEV),
+                torch.zeros((1, N, r), dtype=dtype, device=DEV))
+
+    y, x, a, b = zeros(torch.float16, 2)
+    x[:], a[:] = 1.0, 1.0
+    x[:, 1], a[0, 0, 0], a[0, 1, 1] = 6e4, math.inf, 6e4
+    b[0, :, 0], b[0, :, 1] = 1.0, -1.0
+    assert (adapters.add_low_rank(y, x, a, b, ids) == math.inf).all()
+    y, x, a, b = zeros(torch.bfloat16, 1)
+    x[:, 0], x[:, 1] = torch.finfo(torch.bfloat16).max, 2.0 ** 119 + 2.0 ** 118
+    a[0, 0, :2], b[:] = 1.0, 2.0 ** -100
+    v = x[0, 0].double() + x[0, 1].double()
+    got = adapters.add_low_rank(y, x, a, b, ids)
+    assert torch.equal(got, (v * 2.0 ** -100).to(torch.bfloat16).expand(M, N))
+    # Low-rank values of one bit, of none, and far below the row's largest, times infinity.
+    for dtype in TYPES:
+        for value, want in ((1.0, math.inf), (-2.0 ** -14, -math.inf), (0.0, math.nan)):
+            for beside in (0.0, 2.0 ** 15):
+                y, x, a, b = zeros(dtype, 3)
+                x[:, 0], x[:, 1] = 1.0, beside
+                a[0, 1, 0], a[0, 0, 1], b[0, :, 1] = value, 2.0 ** 10, math.inf
+                got = adapters.add_low_rank(y, x, a, b, ids)
+                assert torch.equal(classes(got), classes(torch.full_like(got, want)))

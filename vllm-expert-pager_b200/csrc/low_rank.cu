@@ -81,6 +81,7 @@ struct Half;
 template <>
 struct Half<__nv_bfloat16> {
   static constexpr bool kNarrowRange = false;
+  static constexpr float kLeast = 0x1p-133f;  // above 0
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t *>(&h);
@@ -105,6 +106,7 @@ struct Half<__nv_bfloat16> {
 template <>
 struct Half<__half> {
   static constexpr bool kNarrowRange = true;
+  static constexpr float kLeast = 0x1p-24f;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<uint32_t *>(&h);
@@ -133,24 +135,33 @@ __device__ __forceinline__ void narrow(__nv_bfloat16 *p, float x) { *p = __float
 __device__ __forceinline__ void narrow(__half *p, float x) { *p = __float2half_rn(x); }
 
 // The parts of two neighbouring values, cut and not rounded, so that each is exact and
-// none leaves the range.  Of what is not finite the first part holds all.
+// none leaves the range.  All have the value's sign and none is 0 unless the value is (the
+// type's least value stands instead, below the last bit of any sum here), so that an
+// infinity of B times the parts is the infinity that it is times the value, and no NaN.  Of
+// an infinity or NaN the first part holds all.
 template <typename T>
 __device__ __forceinline__ void split(float u, float w, uint32_t (&part)[3]) {
+  const uint32_t sign = (__float_as_uint(u) >> 16 & 0x8000u) | (__float_as_uint(w) & 0x80000000u);
+  const float u0 = u == 0.0f ? 0.0f : Half<T>::kLeast, w0 = w == 0.0f ? 0.0f : Half<T>::kLeast;
+  u = fabsf(u), w = fabsf(w);
+  u = u < u0 ? u0 : u, w = w < w0 ? w0 : w;  // a NaN stays
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
-    part[i] = Half<T>::cut(u, w);
-    const float2 h = Half<T>::unpack(part[i]);
-    u = isfinite(h.x) ? u - h.x : 0.0f, w = isfinite(h.y) ? w - h.y : 0.0f;
+    const uint32_t q = Half<T>::cut(u, w);
+    const float2 h = Half<T>::unpack(q);
+    part[i] = q | sign;
+    u = fmaxf(u - h.x, u0), w = fmaxf(w - h.y, w0);
   }
 }
 
-// The power of two that brings a row's largest magnitude into [2^14, 2^15); 1 for
-// rows of zeros (or less than 2^-126), of infinities and of NaN.
+// The power of two that brings a row's largest magnitude (of the finite values) into
+// [2^14, 2^15), 2^126 at most.
 __device__ __forceinline__ float range_factor(float amax) {
   const int e = static_cast<int>(__float_as_uint(amax) >> 23);  // the biased exponent
-  return e == 0 || e == 255 ? 1.0f
-                            : __uint_as_float(static_cast<uint32_t>(min(268 - e, 253)) << 23);
+  return __uint_as_float(static_cast<uint32_t>(min(268 - e, 253)) << 23);
 }
+
+__device__ __forceinline__ float finite_abs(float x) { return isfinite(x) ? fabsf(x) : 0.0f; }
 
 // The slot of row m, -1 without an adapter.
 __device__ __forceinline__ int slot_of_row(const LowRankArgs &a, int64_t m) {
@@ -537,8 +548,12 @@ __global__ void __launch_bounds__(kThreads, kVec && kRB <= 4 ? 3 : 2)
       float f = 1.0f;
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
-        u[i][0] *= scale, u[i][1] *= scale;
-        amax = fmaxf(amax, fmaxf(fabsf(u[i][0]), fabsf(u[i][1])));
+        // Behind the last rank stands 0, whatever x is (an infinity times 0 is none).
+        const int e = i * 64 + 2 * lane;
+        u[i][0] = e < a.r ? u[i][0] * scale : 0.0f;
+        u[i][1] = e + 1 < a.r ? u[i][1] * scale : 0.0f;
+        if (Half<T>::kNarrowRange)
+          amax = fmaxf(amax, fmaxf(finite_abs(u[i][0]), finite_abs(u[i][1])));
       }
       if constexpr (Half<T>::kNarrowRange)
         f = range_factor(__uint_as_float(__reduce_max_sync(kFull, __float_as_uint(amax))));
@@ -1342,16 +1357,18 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
       }
     }
     float f = 1.0f;
+    // Behind the last rank stands 0, whatever x is (an infinity times 0 is none).
 #pragma unroll
     for (int i = 0; i < kMine; ++i)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) u[i][j] *= scale;
+      for (int j = 0; j < 16; ++j)
+        u[i][j] = (2 * i + side) * 16 + j < a.r ? u[i][j] * scale : 0.0f;
     if constexpr (Half<T>::kNarrowRange) {
       float most = 0.0f;
 #pragma unroll
       for (int i = 0; i < kMine; ++i)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(u[i][j]));
+        for (int j = 0; j < 16; ++j) most = fmaxf(most, finite_abs(u[i][j]));
       amax[side][row] = most;
       asm volatile("bar.sync 1, 256;" ::: "memory");
       f = range_factor(fmaxf(amax[0][row], amax[1][row]));
