@@ -404,3 +404,40 @@ def test_refusals_on_the_device():
         routing.route(logits, 2, valid=torch.ones((4,), dtype=torch.bool))
     with pytest.raises(ValueError, match="expected a CUDA tensor"):
         routing.balance_loss(logits, torch.zeros((4, 2), dtype=torch.int32))
+
+
+@pytest.mark.parametrize("T, E", [(1 << 26, 5), (1 << 25, 50), (1 << 24, 200), (1 << 23, 300),
+                                  (1 << 22, 800), (1 << 21, 1100), (1 << 20, 4096)])
+def test_mean_probabilities_of_long_batches(T, E):
+    """P adds up 2^26 tokens as exactly as a few: one row for all tokens, so that every
+    addition rounds the same way.  32 tokens are summed in 32 bits, those sums in 64."""
+    from vllm_expert_pager import routing
+
+    row, _ = make(1, E, torch.float32, seed=E)
+    logits = row.expand(T, E)
+    p, x = softmax64(row.double(), torch.ones((1,), dtype=torch.bool, device=DEV))
+    rel = (float(steps(x.abs().max(), E)) + 40) * STEP
+    if E <= 200:
+        top = int(row.argmax())
+        r = routing.route(logits, 1, balance=True)
+        assert int(r.counts[top]) == T and int(r.counts.sum()) == T
+        want = E * float(p[0, top])
+        assert abs(float(r.loss) - want) <= rel * want
+        del r
+    ids = torch.full((T, 1), E // 2, dtype=torch.int32, device=DEV)
+    loss, counts = routing.balance_loss(logits, ids)
+    assert int(counts[E // 2]) == T
+    want = E * float(p[0, E // 2])
+    assert abs(float(loss) - want) <= rel * want
+
+
+@pytest.mark.parametrize("E", [50, 256, 1100])
+def test_rows_without_an_open_expert_in_a_long_batch(E):
+    """Rows that add nothing to P, and rows that hold no token, wherever a warp's sum moves on
+    to 64 bits."""
+    T = 200000
+    logits, g = make(T, E, torch.bfloat16, seed=E)
+    logits[torch.rand((T,), generator=g, device=DEV) < 0.3] = -math.inf
+    valid = torch.rand((T,), generator=g, device=DEV) < 0.7
+    for v in (None, valid):
+        check_route(logits, 3, False, valid=v)

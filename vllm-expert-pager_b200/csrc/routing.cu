@@ -16,9 +16,10 @@
 // reads are whole 16-byte vectors.  For the choice a lane's logits become integers
 // that hold their order and their expert (see Choice), sorted in registers; each of
 // the k steps then takes the largest first one of the lanes' runs.  Sums over tokens (P, c) are kept per lane
-// over a warp's tokens, added over the CTA's warps in their order, and over the
-// CTAs in theirs by a second small launch: no atomics on floats, so the loss does
-// not depend on the order in which CTAs run.
+// over a warp's tokens (P's 32 bits hold 32 tokens at most, then 64 bits take them: over
+// 2^26 tokens 32 bits lose 1e-4 of P), added over the CTA's warps in their order, and over
+// the CTAs in theirs by a second small launch: no atomics on floats, so the loss does not
+// depend on the order in which CTAs run.
 //
 // Few experts or tokens: bound by latency (one token of 256 experts 3.4 us).  Many:
 // the loss of 65536 x 512 logits in 32 bits reads 134 MB in 38 us at 56 % of the
@@ -41,6 +42,7 @@ namespace cg = cooperative_groups;
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kSumCtas = 8;       // CTAs (one cluster) of the sum over CTAs
 constexpr int kSumThreads = 1024;
+constexpr int kFold = 32;         // tokens whose probabilities are summed in 32 bits
 constexpr int kMaxCtas = 444;     // most CTAs of the forward kernel (3 for each of 148 SMs)
 
 // Threads of a CTA of the forward kernel and CTAs on an SM, by the values per lane:
@@ -194,6 +196,11 @@ struct Row {
     return ((i / kV) * 32 + lane) * kV + i % kV;
   }
 
+  // Where an expert's sum stands in a row of sums, and such a row's length: skewed so that
+  // neither the lanes' values of one register nor neighbouring experts share banks.
+  static __device__ __forceinline__ int place(int e) { return kV > 1 ? e + e / kV : e; }
+  static constexpr int kPlaces = 32 * VPL + (kV > 1 ? 32 * VPL / kV : 0);
+
   // A row in two steps, so that the next one can be on its way.  Places past the
   // row's end hold -inf from the start; no fetch touches them.
   struct Raw {
@@ -297,17 +304,25 @@ struct ForwardArgs {
   int64_t *counts;  // [E]
   int64_t *tokens;  // the tokens that count (may be NULL)
   float *loss;      // NULL: no balance loss
-  // One row per CTA, for the sum over CTAs: P, c, n.
-  float *part_p;
-  int32_t *part_c, *part_n;
+  // One row per CTA, for the sum over CTAs: P (its 64 bits in two words), c, n.
+  int32_t *part_p, *part_q, *part_c, *part_n;
 };
 
-// The loss and the outputs from totals of one block of experts; returns the
-// block's share of sum_e f_e P_e.
-__device__ __forceinline__ float finish(const ForwardArgs &a, int e, float p, int c, int n) {
+// Writes the count of an expert; returns its share of n^2 k sum_e f_e P_e.
+__device__ __forceinline__ double finish(const ForwardArgs &a, int e, double p, int c) {
   a.counts[e] = c;
-  if (n == 0) return 0.0f;
-  return (static_cast<float>(c) / (static_cast<float>(n) * a.topk)) * (p / n);
+  return c * p;
+}
+
+__device__ __forceinline__ float loss_of(const ForwardArgs &a, double s, int n) {
+  return n == 0 ? 0.0f
+                : static_cast<float>(a.E * s / (static_cast<double>(n) * n * a.topk));
+}
+
+__device__ __forceinline__ double warp_sum(double x) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(kFull, x, o);
+  return x;
 }
 
 // kGiven: the ids were chosen elsewhere.
@@ -322,16 +337,18 @@ __global__ void __launch_bounds__(forward_threads(VPL), forward_blocks(VPL))
   const int E = a.E, warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool balance = a.loss != nullptr;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  int *cnt = reinterpret_cast<int *>(smem);               // [E]
-  float *sum = reinterpret_cast<float *>(smem) + E;       // [E], or [warps][E]
+  // The sums of p in 64 bits, a row for each warp (one row in all where the rows below
+  // are); those in 32 bits; the counts.
+  double *total = reinterpret_cast<double *>(smem);
+  float *sum = reinterpret_cast<float *>(
+      total + (!balance ? 0 : (kAccShared ? E : warps * R::kPlaces)));
+  int *cnt = reinterpret_cast<int *>(sum + (balance && kAccShared ? warps * E : 0));
   __shared__ int tokens;
-  __shared__ float loss_part[16];
+  __shared__ double loss_part[16];
 
   for (int e = threadIdx.x; e < E; e += blockDim.x) cnt[e] = 0;
-  if (balance) {
-    const int rows = kAccShared ? warps : 1;
-    for (int e = threadIdx.x; e < rows * E; e += blockDim.x) sum[e] = 0.0f;
-  }
+  if (balance && kAccShared)
+    for (int e = threadIdx.x; e < warps * E; e += blockDim.x) sum[e] = 0.0f;
   if (threadIdx.x == 0) tokens = 0;
   __syncthreads();
 
@@ -340,7 +357,27 @@ __global__ void __launch_bounds__(forward_threads(VPL), forward_blocks(VPL))
 #pragma unroll
     for (int i = 0; i < VPL; ++i) acc[i] = 0.0f;
   }
-  int mine = 0;  // tokens of this warp that count
+  // What the 32 bits hold goes to the 64: of a warp by itself, or (rows in shared memory)
+  // of all warps together.
+  auto fold = [&](bool folded) {  // before this time
+    if constexpr (kAccShared) {
+      __syncthreads();
+      for (int e = threadIdx.x; e < E; e += blockDim.x) {
+        double s = folded ? total[e] : 0.0;
+        for (int w = 0; w < warps; ++w) s += sum[w * E + e], sum[w * E + e] = 0.0f;
+        total[e] = s;
+      }
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        double *at = total + warp * R::kPlaces + R::place(R::expert(i, lane));
+        *at = folded ? *at + acc[i] : acc[i];
+        acc[i] = 0.0f;
+      }
+    }
+  };
+  int mine = 0, rounds = 0;  // tokens of this warp that count; the CTA's rounds
   const int64_t step = static_cast<int64_t>(gridDim.x) * warps;
   int64_t t = static_cast<int64_t>(blockIdx.x) * warps + warp;
   // A token's row is fetched while the one before it is worked on, its flag one
@@ -351,7 +388,9 @@ __global__ void __launch_bounds__(forward_threads(VPL), forward_blocks(VPL))
   typename R::Raw raw;
   bool live = counts(t), next_live = counts(t + step);
   if (live) R::fetch(row_of(t), E, lane, raw);
-  for (; t < a.T; t += step) {
+  // As many rounds for all of the CTA's warps, where they fold together.
+  for (int64_t t0 = kAccShared ? t - warp : t; t0 < a.T; t0 += step, t += step) {
+    if (kAccShared && balance && rounds++ % kFold == 0 && rounds > 1) fold(rounds > kFold + 1);
     float v[VPL];
     const bool here = live;
     if (here) R::open(raw, v);
@@ -361,7 +400,7 @@ __global__ void __launch_bounds__(forward_threads(VPL), forward_blocks(VPL))
       if (live) R::fetch(row_of(t + step), E, lane, raw);
     }
     if (!here) {
-      if (!kGiven && lane < a.topk) {
+      if (!kGiven && t < a.T && lane < a.topk) {
         a.weights[t * a.topk + lane] = 0.0f;
         a.ids[t * a.topk + lane] = -1;
       }
@@ -404,6 +443,7 @@ __global__ void __launch_bounds__(forward_threads(VPL), forward_blocks(VPL))
         }
       }
     }
+    if (!kAccShared && balance && mine % kFold == 0) fold(mine > kFold);
     // Where two rows do not fit the registers the next one is fetched at the end.
     if (!kAhead) next_live = counts(t + 2 * step);
     if constexpr (kGiven) {
@@ -480,29 +520,27 @@ __global__ void __launch_bounds__(forward_threads(VPL), forward_blocks(VPL))
   }
 
   if (lane == 0 && mine) atomicAdd(&tokens, mine);
-  if (balance && !kAccShared) {
-    for (int w = 0; w < warps; ++w) {
-      __syncthreads();
-      if (w == warp) {
-#pragma unroll
-        for (int i = 0; i < (kAccShared ? 1 : VPL); ++i) {
-          const int e = R::expert(i, lane);
-          if (e < E) sum[e] += acc[i];
-        }
+  if (balance) fold(kAccShared ? rounds > kFold : mine >= kFold);
+  __syncthreads();
+  double part = 0.0;
+  for (int e = threadIdx.x; e < E; e += blockDim.x) {
+    double p = 0.0;
+    if (balance) {
+      if constexpr (kAccShared) {
+        p = total[e];
+      } else {
+        for (int w = 0; w < warps; ++w) p += total[w * R::kPlaces + R::place(e)];
       }
     }
-  }
-  __syncthreads();
-  float part = 0.0f;
-  for (int e = threadIdx.x; e < E; e += blockDim.x) {
-    float p = 0.0f;
-    if (balance)
-      for (int w = 0; w < (kAccShared ? warps : 1); ++w) p += sum[w * E + e];
     if (gridDim.x == 1) {
-      part += finish(a, e, p, cnt[e], tokens);
+      part += finish(a, e, p, cnt[e]);
     } else {
-      a.part_c[static_cast<int64_t>(blockIdx.x) * E + e] = cnt[e];
-      if (balance) a.part_p[static_cast<int64_t>(blockIdx.x) * E + e] = p;
+      const int64_t at = static_cast<int64_t>(blockIdx.x) * E + e;
+      a.part_c[at] = cnt[e];
+      if (balance) {
+        a.part_p[at] = __double2hiint(p);
+        a.part_q[at] = __double2loint(p);
+      }
     }
   }
   if (gridDim.x > 1) {
@@ -515,9 +553,9 @@ __global__ void __launch_bounds__(forward_threads(VPL), forward_blocks(VPL))
   if (lane == 0) loss_part[warp] = part;
   __syncthreads();
   if (threadIdx.x == 0) {
-    float s = 0.0f;
+    double s = 0.0;
     for (int w = 0; w < warps; ++w) s += loss_part[w];
-    *a.loss = s * E;
+    *a.loss = loss_of(a, s, tokens);
   }
 }
 
@@ -526,9 +564,9 @@ __global__ void __launch_bounds__(forward_threads(VPL), forward_blocks(VPL))
 // loss through distributed shared memory.
 __global__ void __cluster_dims__(kSumCtas, 1, 1) __launch_bounds__(kSumThreads)
     sum_kernel(const __grid_constant__ ForwardArgs a, int rows) {
-  __shared__ float sp[kSumThreads];
+  __shared__ double sp[kSumThreads];
   __shared__ int sc[kSumThreads];
-  __shared__ float block_loss;
+  __shared__ double block_loss;
   __shared__ int tokens;
   cg::cluster_group cluster = cg::this_cluster();
   const int E = a.E, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -541,32 +579,42 @@ __global__ void __cluster_dims__(kSumCtas, 1, 1) __launch_bounds__(kSumThreads)
   if (lane == 0) atomicAdd(&tokens, n);
   __syncthreads();
   n = tokens;
-  float loss = 0.0f;
+  double loss = 0.0;
   constexpr int kCols = 32, kGroups = kSumThreads / kCols;
   constexpr int kEach = (kMaxCtas + kGroups - 1) / kGroups;
   for (int e0 = blockIdx.x * kCols; e0 < E; e0 += kSumCtas * kCols) {
     const int e = e0 + lane;
-    float q[kEach];
-    int d[kEach];
+    int hi[kEach], lo[kEach], d[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {  // all of a thread's loads under way at once
       const int r = warp + i * kGroups;
       const bool in = e < E && r < rows;
-      d[i] = in ? a.part_c[static_cast<int64_t>(r) * E + e] : 0;
-      q[i] = in && balance ? a.part_p[static_cast<int64_t>(r) * E + e] : 0.0f;
+      const int64_t at = static_cast<int64_t>(r) * E + e;
+      d[i] = in ? a.part_c[at] : 0;
+      hi[i] = in && balance ? a.part_p[at] : 0;
+      lo[i] = in && balance ? a.part_q[at] : 0;
     }
-    float p = 0.0f;
+    double p[2] = {0.0, 0.0};  // two chains of additions
     int c = 0;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) p += q[i], c += d[i];
+    for (int i = 0; i < kEach; ++i) c += d[i];
+    if (balance)
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) p[i & 1] += __hiloint2double(hi[i], lo[i]);
     __syncthreads();
-    sp[tid] = p;
+    if (balance) sp[tid] = p[0] + p[1];
     sc[tid] = c;
     __syncthreads();
     if (warp == 0 && e < E) {
 #pragma unroll 8
-      for (int g = 1; g < kGroups; ++g) p += sp[g * kCols + lane], c += sc[g * kCols + lane];
-      loss += finish(a, e, p, c, n);
+      for (int g = 1; g < kGroups; ++g) c += sc[g * kCols + lane];
+      double q[4] = {0.0, 0.0, 0.0, 0.0};
+      if (balance)
+#pragma unroll 2
+        for (int g = 0; g < kGroups; g += 4)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) q[k] += sp[(g + k) * kCols + lane];
+      loss += finish(a, e, (q[0] + q[1]) + (q[2] + q[3]), c);
     }
   }
   if (blockIdx.x == 0 && tid == 0 && a.tokens) *a.tokens = n;
@@ -575,9 +623,9 @@ __global__ void __cluster_dims__(kSumCtas, 1, 1) __launch_bounds__(kSumThreads)
   if (tid == 0) block_loss = loss;
   cluster.sync();
   if (blockIdx.x == 0 && tid == 0) {
-    float s = 0.0f;
+    double s = 0.0;
     for (int b = 0; b < kSumCtas; ++b) s += *cluster.map_shared_rank(&block_loss, b);
-    *a.loss = s * E;
+    *a.loss = loss_of(a, s, n);
   }
   cluster.sync();  // the blocks' shared memory stays until it has been read
 }
@@ -730,8 +778,10 @@ int launch_forward(const ForwardArgs &a, cudaStream_t s) {
   auto fn = a.given ? forward_kernel<T, VPL, VEC, true> : forward_kernel<T, VPL, VEC, false>;
   const int threads = forward_threads(VPL);
   const int64_t ctas = forward_ctas(a.T, a.E);
-  const int rows = 1 + (a.loss ? (VPL > 32 ? threads / 32 : 1) : 0);
-  const size_t smem = sizeof(float) * a.E * rows;
+  size_t smem = sizeof(int) * a.E;
+  if (a.loss)
+    smem += VPL > 32 ? (sizeof(double) + sizeof(float) * (threads / 32)) * a.E
+                     : sizeof(double) * (threads / 32) * Row<T, VPL, VEC>::kPlaces;
   int rc = set_smem((const void *)fn, smem);
   if (rc) return rc;
   fn<<<static_cast<unsigned>(ctas), threads, smem, s>>>(a);
@@ -822,7 +872,7 @@ int check_sizes(int dtype, int64_t T, int64_t E, int64_t stride, int64_t topk) {
 
 int64_t scratch_need(int64_t T, int64_t E) {
   const int64_t ctas = forward_ctas(T, E);
-  return ctas == 1 ? 0 : ctas * (E * 8 + 4);
+  return ctas == 1 ? 0 : ctas * (E * 12 + 4);
 }
 
 int run_forward(ForwardArgs &a, int dtype, void *scratch, int64_t scratch_bytes, void *stream) {
@@ -830,8 +880,9 @@ int run_forward(ForwardArgs &a, int dtype, void *scratch, int64_t scratch_bytes,
   if (ctas > 1) {
     if (!scratch || !aligned(scratch, 4) || scratch_bytes < scratch_need(a.T, a.E))
       return XP_EINVAL;
-    a.part_p = static_cast<float *>(scratch);
-    a.part_c = reinterpret_cast<int32_t *>(a.part_p + ctas * a.E);
+    a.part_p = static_cast<int32_t *>(scratch);
+    a.part_q = a.part_p + ctas * a.E;
+    a.part_c = a.part_q + ctas * a.E;
     a.part_n = a.part_c + ctas * a.E;
   }
   return by_type<ForwardArgs, Forward>(a, dtype, nullptr, as_stream(stream));
@@ -857,7 +908,7 @@ extern "C" int xp_route(const void *logits, int dtype, int64_t T, int64_t E, int
   if (topk > XP_MAX_TOPK) return XP_ERANGE;
   if (!counts || (T > 0 && (!logits || !weights || !ids))) return XP_EINVAL;
   ForwardArgs a{logits, T, stride, static_cast<int>(E), static_cast<int>(topk), renormalize, valid,
-                weights, ids, nullptr, 4, counts, tokens, loss, nullptr, nullptr, nullptr};
+                weights, ids, nullptr, 4, counts, tokens, loss, nullptr, nullptr, nullptr, nullptr};
   return run_forward(a, dtype, scratch, scratch_bytes, stream);
 }
 
@@ -873,7 +924,7 @@ extern "C" int xp_balance(const void *logits, int dtype, int64_t T, int64_t E, i
   // An empty batch has no ids to point at; the kernel then reads none.
   ForwardArgs a{logits, T, stride, static_cast<int>(E), static_cast<int>(topk), 0, valid,
                 nullptr, nullptr, T > 0 ? ids : counts, ids_bytes, counts, tokens, loss, nullptr,
-                nullptr, nullptr};
+                nullptr, nullptr, nullptr};
   return run_forward(a, dtype, scratch, scratch_bytes, stream);
 }
 
