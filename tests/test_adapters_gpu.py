@@ -566,3 +566,34 @@ def test_values_beside_an_infinity_and_at_the_range_end(M):
                 a[0, 1, 0], a[0, 0, 1], b[0, :, 1] = value, 2.0 ** 10, math.inf
                 got = adapters.add_low_rank(y, x, a, b, ids)
                 assert torch.equal(classes(got), classes(torch.full_like(got, want)))
+
+
+@pytest.mark.parametrize("M", [3, 1100])
+def test_autograd_sees_the_update_in_place(M):
+    """A value that autograd has saved may not change unseen, as with torch's own updates."""
+    from vllm_expert_pager import adapters
+
+    o, _ = make(M, 64, 32, 8, 2, torch.bfloat16)
+    ids = torch.zeros((M,), dtype=torch.int32, device=DEV)
+    gate = torch.ones((M, 32), dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    for out in (None, "out"):
+        t = o["y"] if out is None else torch.zeros_like(o["y"])
+        z = t * gate
+        before = t._version
+        adapters.add_low_rank(o["y"], o["x"], o["a"], o["b"], ids, out=None if out is None else t)
+        assert t._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.sum().backward()
+    h = gate.exp()  # saves its result
+    with torch.no_grad():
+        adapters.add_low_rank(h, o["x"], o["a"], o["b"], ids)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        h.sum().backward()
+    # What is only read stays as it was, and tensors without a version are taken as before.
+    versions = [o[k]._version for k in ("x", "a", "b", "y")]
+    adapters.add_low_rank(o["y"], o["x"], o["a"], o["b"], ids, out=torch.empty_like(o["y"]))
+    assert versions == [o[k]._version for k in ("x", "a", "b", "y")]
+    with torch.inference_mode():
+        y = o["y"].clone()
+    want = adapters.add_low_rank(o["y"], o["x"], o["a"], o["b"], ids, out=torch.empty_like(o["y"]))
+    assert torch.equal(adapters.add_low_rank(y, o["x"], o["a"], o["b"], ids), want)

@@ -342,6 +342,9 @@ Tensor add_low_rank(const Tensor &y_in, const Tensor &x_in, const Tensor &a, con
   const Tensor ids = ids_in.contiguous();
   const Tensor scale = scale_in ? scale_in->contiguous() : Tensor();
   const Tensor map = map_in ? map_in->contiguous() : Tensor();
+  // out changes under autograd's eyes, as by torch's own updates in place: a backward pass
+  // that saved its old values then raises.
+  if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
   const int64_t need = xp_low_rank_scratch_bytes(M, S);
   Tensor scratch;
   if (need > 0) scratch = at::empty({need}, x.options().dtype(at::kByte).requires_grad(false));
