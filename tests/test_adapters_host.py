@@ -149,3 +149,16 @@ def test_columns_of_one_buffer_do_not_overlap():
 def test_pager_refuses_its_arguments(args, words):
     with pytest.raises(ValueError, match=words):
         adapters.AdapterPager(*args, torch.device("cpu"))
+
+
+def test_dual_tensors_are_refused():
+    from torch.autograd import forward_ad
+
+    with forward_ad.dual_level():
+        for name in ("x", "y", "a", "b", "scale", "out"):
+            o = {**operands(), "scale": torch.ones((3,)), "out": torch.zeros((6, 24)).bfloat16()}
+            o[name] = forward_ad.make_dual(o[name], torch.ones_like(o[name]))
+            with pytest.raises(ValueError, match="no forward-mode derivative"):
+                adapters.add_low_rank(**o)
+        with pytest.raises(ValueError, match="expected a CUDA tensor"):
+            adapters.add_low_rank(**operands())

@@ -121,3 +121,22 @@ def test_balance_refusals():
     with pytest.raises(ValueError, match="valid must be"):
         routing.balance_loss(x, torch.zeros((4, 2), dtype=torch.int32),
                              valid=torch.ones((3,), dtype=torch.bool))
+
+
+def test_dual_tensors_are_refused():
+    """A tangent would be lost in silence; where forward-mode derivatives are off it is no
+    matter, and the call gets as far as the device."""
+    from torch.autograd import forward_ad
+
+    ids = torch.zeros((4, 2), dtype=torch.int32)
+    with forward_ad.dual_level():
+        for leaf in (torch.ones((4, 8)), torch.ones((4, 8), requires_grad=True)):
+            x = forward_ad.make_dual(leaf, torch.ones((4, 8)))
+            for call in (lambda: routing.route(x, 2), lambda: routing.balance_loss(x, ids)):
+                with pytest.raises(ValueError, match="no forward-mode derivative"):
+                    call()
+                with forward_ad._set_fwd_grad_enabled(False):
+                    with pytest.raises(ValueError, match="expected a CUDA tensor"):
+                        call()
+        with pytest.raises(ValueError, match="expected a CUDA tensor"):
+            routing.route(torch.ones((4, 8)), 2)

@@ -6,6 +6,7 @@
 // B200 host a route of one token took 18 us and a balance loss with its gradient 99 us,
 // here 9 and 59 (torch's own sum and its gradient: 47).  The Python modules routing.py and
 // adapters.py document the functions; this file keeps their argument checks.
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -50,6 +51,12 @@ void require_cuda(const Tensor &t) {
   require(t.is_cuda(), "vllm-expert-pager: expected a CUDA tensor, got one on ", t.device().str());
 }
 
+// A dual tensor's tangent would be lost, and the result pass for a constant.
+void require_no_tangent(const Tensor &t, const char *what) {
+  require(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(),
+          what, " has no forward-mode derivative");
+}
+
 // A status of libxpager.so as native.check words it.
 void check_status(int rc, const char *what) {
   if (rc == XP_OK) return;
@@ -82,6 +89,7 @@ void check_logits(const Tensor &logits, const MaybeTensor &valid) {
   const int64_t T = logits.size(0), E = logits.size(1);
   require(E >= 1 && E <= XP_MAX_EXPERTS, "between 1 and ", XP_MAX_EXPERTS,
           " experts are supported, got ", E);
+  require_no_tangent(logits, "routing");
   require(T <= XP_MAX_TOKENS, "at most ", XP_MAX_TOKENS, " tokens are supported, got ", T);
   if (valid) {
     require((valid->scalar_type() == at::kBool || valid->scalar_type() == at::kByte) &&
@@ -313,6 +321,8 @@ Tensor add_low_rank(const Tensor &y_in, const Tensor &x_in, const Tensor &a, con
     require(!(x.requires_grad() || y.requires_grad() || a.requires_grad() || b.requires_grad() ||
               out.requires_grad() || (scale_in && scale_in->requires_grad())),
             "add_low_rank has no gradient: call it under torch.no_grad() or on detached tensors");
+  for (const Tensor *v : {&x_in, &y_in, &a, &b, &out}) require_no_tangent(*v, "add_low_rank");
+  if (scale_in) require_no_tangent(*scale_in, "add_low_rank");
   require(a.is_contiguous() && b.is_contiguous(), "adapter slabs must be contiguous");
   require((out.stride(1) == 1 || N == 1) && (out.stride(0) >= N || M <= 1),
           "the rows of out must be contiguous and apart");

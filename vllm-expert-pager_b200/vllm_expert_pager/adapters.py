@@ -39,7 +39,8 @@ def add_low_rank(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     (the update in place) and may share no memory with the other operands.
     Ranks up to 128; pad an adapter of a lower rank with zeros.  The sums are
     held in 32 bits and the result is rounded once.  Not differentiable: a call
-    that would need a gradient is refused, and a backward pass that saved the
+    that would need a gradient, or with a dual tensor of forward-mode
+    derivatives, is refused, and a backward pass that saved the
     values which ``out`` had before raises, as after torch's own updates in place.
     """
     return native.torch_ops().add_low_rank(y, x, a, b, ids, scale, slot_map, out)

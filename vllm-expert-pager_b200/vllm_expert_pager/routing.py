@@ -10,8 +10,8 @@ experts, get them here:
   slots a layer needs); in training also the balance loss.
 * ``balance_loss``: the same loss and counts for a routing chosen elsewhere.
 
-Both are differentiable by the logits, once (a gradient with ``create_graph`` is
-refused).  Each forward and backward pass is one or two launches of
+Both are differentiable by the logits, once and backwards (a gradient with
+``create_graph`` and a dual tensor of forward-mode derivatives are refused).  Each forward and backward pass is one or two launches of
 ``libxpager.so`` (routing.cu) on the current stream of the tensors' device,
 without a host synchronisation, so they can be captured in a CUDA graph.
 Arguments are checked in csrc/torch_ops.cpp; a refused call raises ValueError
