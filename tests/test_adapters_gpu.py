@@ -597,3 +597,58 @@ def test_autograd_sees_the_update_in_place(M):
         y = o["y"].clone()
     want = adapters.add_low_rank(o["y"], o["x"], o["a"], o["b"], ids, out=torch.empty_like(o["y"]))
     assert torch.equal(adapters.add_low_rank(y, o["x"], o["a"], o["b"], ids), want)
+
+
+def test_add_follows_a_replayed_page():
+    """A captured page that is replayed after an eager one moves adapters: the add behind it
+    reads the slots that are current, eagerly and in a graph of its own."""
+    num, S, rank, H, N, dtype = 12, 3, 8, 64, 48, torch.bfloat16
+    pager, all_, g = pager_of(num, S, rank, H, N, dtype, seed=5)
+    try:
+        a, b, f = slabs(all_, rank, H, N, dtype)
+        requests = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV)
+        pager.page(requests)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            pager.page(requests)
+        M = 9
+        y = torch.randn((M, N), generator=g).to(dtype).to(DEV)
+        x = torch.randn((M, H), generator=g).to(dtype).to(DEV)
+        rows = torch.zeros((M,), dtype=torch.int32, device=DEV)
+        out = torch.empty_like(y)
+        pager.add(y, x, rows, out=out)
+        torch.cuda.synchronize()
+        adds = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(adds):
+            pager.add(y, x, rows, out=out)
+        for step in range(6):
+            pager.page(torch.randperm(num, generator=g)[:S].to(DEV))
+            new = torch.randperm(num, generator=g)[:S]
+            requests.copy_(new)
+            graph.replay()
+            ids = new[torch.randint(0, S, (M,), generator=g)].to(DEV)
+            rows.copy_(ids)
+            want, bound = reference(y, x, a, b, ids, f)
+            got = pager.add(y, x, ids, out=torch.empty_like(y))
+            assert ((got.double() - want).abs() <= bound).all(), step
+            adds.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, got)
+        # New weights: the rows of the adapter keep y until it is paged again.
+        i = int(new[0])
+        rows.fill_(i)
+        all_[i] = adapter(i, rank, H, N, dtype, g)
+        pager.write(i, *all_[i])
+        assert torch.equal(pager.add(y, x, rows, out=torch.empty_like(y)), y)
+        pager.page(rows[:1])
+        a, b, f = slabs(all_, rank, H, N, dtype)
+        want, bound = reference(y, x, a, b, rows.long(), f)
+        got = pager.add(y, x, rows, out=torch.empty_like(y))
+        assert ((got.double() - want).abs() <= bound).all()
+        # The number behind the last adapter is no adapter.
+        last = torch.full((M,), num, dtype=torch.int32, device=DEV)
+        assert torch.equal(pager.add(y, x, last, out=torch.empty_like(y)), y)
+        del graph, adds
+    finally:
+        pager.release()

@@ -149,14 +149,18 @@ class AdapterPager:
             if todo.numel():
                 gather_rows(todo, slot, self.table.no_cache, self.table.experts, 0, self._rows,
                             self._slabs, self._slabs, None, self._scale_rows, self._scale_slots)
-        self.slot_map = slot
+        # The table's own map, not this step's copy: it is current after any page, one
+        # replayed from a graph too.  (Behind the adapters stands the table's sink.)
+        self.slot_map = self.table.slot_of[: self.num_adapters]
         return slot
 
     def add(self, y: torch.Tensor, x: torch.Tensor, ids: torch.Tensor,
             out: torch.Tensor | None = None) -> torch.Tensor:
         """``add_low_rank`` with every row's adapter id, after ``page`` of the step's adapters.
 
-        A row whose adapter is in no slot keeps ``y``, as a row without one does.
+        The slots are those of the last ``page`` on the device, called or replayed.  A row
+        whose adapter is in no slot (after ``write`` it is in none until the next ``page``)
+        keeps ``y``, as a row without one does.
         """
         if not hasattr(self, "slot_map"):
             raise RuntimeError("vllm-expert-pager: page the step's adapters first")
