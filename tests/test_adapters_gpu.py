@@ -652,3 +652,15 @@ def test_add_follows_a_replayed_page():
         del graph, adds
     finally:
         pager.release()
+
+
+@pytest.mark.parametrize("M", [3, 1100])
+def test_an_empty_slot_map_has_no_adapter(M):
+    from vllm_expert_pager import adapters
+
+    o, _ = make(M, 64, 32, 8, 2, torch.bfloat16)
+    ids = torch.zeros((M,), dtype=torch.int32, device=DEV)
+    for t in (torch.int32, torch.int64):
+        got = adapters.add_low_rank(o["y"], o["x"], o["a"], o["b"], ids, out=fresh(o),
+                                    slot_map=torch.empty((0,), dtype=t, device=DEV))
+        assert torch.equal(got, o["y"])

@@ -352,6 +352,9 @@ Tensor add_low_rank(const Tensor &y_in, const Tensor &x_in, const Tensor &a, con
   const Tensor ids = ids_in.contiguous();
   const Tensor scale = scale_in ? scale_in->contiguous() : Tensor();
   const Tensor map = map_in ? map_in->contiguous() : Tensor();
+  // A map of no adapters has no storage, and is still a map: no row has an adapter.  Nothing
+  // is read from where it points.
+  const void *slot_of = map.defined() && map.numel() == 0 ? ptr(ids) : ptr(map);
   // out changes under autograd's eyes, as by torch's own updates in place: a backward pass
   // that saved its old values then raises.
   if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
@@ -361,7 +364,7 @@ Tensor add_low_rank(const Tensor &y_in, const Tensor &x_in, const Tensor &a, con
   check_status(
       xp_add_low_rank(ptr(x), x.stride(0), ptr(y), y.stride(0), ptr(out), out.stride(0),
                       type_code(t), M, H, N, r, ptr(a), ptr(b), S, ptr<float>(scale), ptr(ids),
-                      static_cast<int>(ids.element_size()), ptr(map),
+                      static_cast<int>(ids.element_size()), slot_of,
                       map.defined() ? static_cast<int>(map.element_size()) : 0,
                       map.defined() ? map.size(0) : 0, ptr(scratch), need, stream_of(x)),
       "add_low_rank");
