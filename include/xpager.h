@@ -354,7 +354,7 @@ int xp_route_backward(const void *logits, int dtype, int64_t T, int64_t E, int64
  * adapter: out[m] = y[m].  x: M rows of H values, y and out: M rows of N values,
  * a: [slots][r][H], b: [slots][N][r] (both contiguous), all of type dtype
  * (XP_BF16 or XP_F16); the strides count elements from row to row.  scale:
- * float[slots], NULL for ones.  out may be y itself (with the same stride) and
+ * float[slots], NULL for ones.  out may be y itself (with the same stride, or of one row) and
  * overlaps no other operand.  r <= XP_MAX_RANK, slots <= XP_MAX_ADAPTER_SLOTS
  * (else XP_ERANGE).  scratch:
  * xp_low_rank_scratch_bytes(M, slots) bytes of device memory, 16-byte aligned

@@ -664,3 +664,20 @@ def test_an_empty_slot_map_has_no_adapter(M):
         got = adapters.add_low_rank(o["y"], o["x"], o["a"], o["b"], ids, out=fresh(o),
                                     slot_map=torch.empty((0,), dtype=t, device=DEV))
         assert torch.equal(got, o["y"])
+
+
+def test_one_row_in_place_at_another_stride():
+    from vllm_expert_pager import adapters
+
+    o, _ = make(1, 64, 48, 8, 2, torch.bfloat16)
+    for slot in (1, -1):
+        ids = torch.full((1,), slot, dtype=torch.int32, device=DEV)
+        want = adapters.add_low_rank(o["y"], o["x"], o["a"], o["b"], ids, out=fresh(o))
+        for offset in (0, 3):
+            buf = torch.full((200,), 7.0, dtype=torch.bfloat16, device=DEV)
+            y = buf.as_strided((1, 48), (100, 1), offset)
+            y.copy_(o["y"])
+            out = buf.as_strided((1, 48), (48, 1), offset)
+            assert adapters.add_low_rank(y, o["x"], o["a"], o["b"], ids, out=out) is out
+            assert torch.equal(out, want)
+            assert (buf[offset + 48 :] == 7.0).all() and (buf[:offset] == 7.0).all()

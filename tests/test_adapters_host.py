@@ -162,3 +162,15 @@ def test_dual_tensors_are_refused():
                 adapters.add_low_rank(**o)
         with pytest.raises(ValueError, match="expected a CUDA tensor"):
             adapters.add_low_rank(**operands())
+
+
+def test_one_row_may_be_updated_in_place_at_any_stride():
+    """The distance to a row that is not there is no difference between out and y."""
+    o = operands(M=1)
+    wide = torch.zeros((2, 64), dtype=torch.bfloat16)
+    for stride in (24, 64, 1000):
+        with pytest.raises(ValueError, match="expected a CUDA tensor"):
+            adapters.add_low_rank(**{**o, "y": wide[:1, :24],
+                                     "out": wide.as_strided((1, 24), (stride, 1))})
+    with pytest.raises(ValueError, match="overlap"):
+        adapters.add_low_rank(**{**o, "y": wide[:1, :24], "out": wide[:1, 1:25]})

@@ -1654,7 +1654,7 @@ extern "C" int xp_add_low_rank(const void *x, int64_t x_stride, const void *y, i
   p.vec_a = aligned(a, 16) && H % 8 == 0;
   p.vec_b = aligned(b, 16) && r % 8 == 0;
   p.vec_y = aligned(y, 16) && aligned(out, 16) && y_stride % 8 == 0 && out_stride % 8 == 0;
-  p.in_place = y == out && y_stride == out_stride;
+  p.in_place = y == out && (y_stride == out_stride || M == 1);
   if (M > kRowsLimit) {
     unsigned char *at = static_cast<unsigned char *>(scratch);
     p.ntiles = reinterpret_cast<int32_t *>(at);

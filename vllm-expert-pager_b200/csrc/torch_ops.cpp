@@ -328,7 +328,7 @@ Tensor add_low_rank(const Tensor &y_in, const Tensor &x_in, const Tensor &a, con
           "the rows of out must be contiguous and apart");
   if (M > 0) {
     const auto at = [](const Tensor &v) { return reinterpret_cast<int64_t>(v.data_ptr()); };
-    const bool same = at(out) == at(y) && out.stride(0) == y.stride(0) &&
+    const bool same = at(out) == at(y) && (out.stride(0) == y.stride(0) || M == 1) &&
                       (out.stride(1) == y.stride(1) || N == 1);
     require(!overlap(at(out), out.stride(0), N, at(x), x.stride(0), H, M) &&
                 (same || !overlap(at(out), out.stride(0), N, at(y), y.stride(0), N, M)),
