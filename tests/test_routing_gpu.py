@@ -441,3 +441,15 @@ def test_rows_without_an_open_expert_in_a_long_batch(E):
     valid = torch.rand((T,), generator=g, device=DEV) < 0.7
     for v in (None, valid):
         check_route(logits, 3, False, valid=v)
+
+
+@pytest.mark.parametrize("E", [7, 200, 1030])
+def test_gradient_where_neighbouring_tokens_choose_the_same_experts(E):
+    """Each token's choices, in another order than those of the tokens that its warp has
+    before and after it: other lanes set the same places."""
+    T, K = 40000, min(E, 32)
+    g = torch.Generator(device=DEV).manual_seed(E)
+    logits = torch.randn((T, E), generator=g, device=DEV) * 0.01
+    logits[:, :K] += 4.0
+    for renormalize in (True, False):
+        check_route(logits, K, renormalize)

@@ -750,6 +750,7 @@ __global__ void __launch_bounds__(kBackThreads, backward_blocks(VPL))
       }
       __syncwarp();
       if (has) sel[id] = 0.0f;
+      __syncwarp();  // another lane may set the same place for the next token
     } else {
 #pragma unroll
       for (int i = 0; i < VPL; ++i) v[i] *= slope(i) - inner;
