@@ -681,3 +681,37 @@ def test_one_row_in_place_at_another_stride():
             assert adapters.add_low_rank(y, o["x"], o["a"], o["b"], ids, out=out) is out
             assert torch.equal(out, want)
             assert (buf[offset + 48 :] == 7.0).all() and (buf[:offset] == 7.0).all()
+
+
+def test_calls_of_several_threads():
+    """Launches of one kernel with other amounts of shared memory, from threads that do not
+    hold the interpreter's lock: none takes away what another has asked for."""
+    import threading
+
+    from vllm_expert_pager import native
+
+    lib = native.lib()
+    M, H, N, r = 1100, 8, 8, 1
+    statuses = {}
+
+    def calls(S, stream, x, y, a, b, ids, scratch):
+        need = lib.xp_low_rank_scratch_bytes(M, S)
+        statuses[S] = {lib.xp_add_low_rank(
+            x.data_ptr(), H, y.data_ptr(), N, y.data_ptr(), N, 1, M, H, N, r, a.data_ptr(),
+            b.data_ptr(), S, None, ids.data_ptr(), 4, None, 0, 0, scratch.data_ptr(), need,
+            stream.cuda_stream) for _ in range(4000)}
+
+    threads = []
+    for S in (4200, 8192):
+        o, _ = make(M, H, N, r, S, torch.bfloat16)
+        ids = torch.full((M,), -1, dtype=torch.int32, device=DEV)
+        scratch = torch.empty((lib.xp_low_rank_scratch_bytes(M, S),), dtype=torch.uint8, device=DEV)
+        threads.append(threading.Thread(target=calls, args=(
+            S, torch.cuda.Stream(), o["x"], o["y"], o["a"], o["b"], ids, scratch)))
+    torch.cuda.synchronize()
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert statuses == {4200: {native.XP_OK}, 8192: {native.XP_OK}}

@@ -14,6 +14,16 @@ inline int launch_status() {
   return err == cudaSuccess ? XP_OK : static_cast<int>(err);
 }
 
+// Lets a launch of fn take `bytes` of dynamic shared memory; `most` is the most that any
+// launch of it takes.  Calls set that one value, so that none of them lowers what another
+// thread has set and not yet launched with.
+inline int allow_smem(const void *fn, int64_t bytes, int64_t most) {
+  if (bytes <= 48 * 1024) return XP_OK;
+  cudaError_t err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(most));
+  return err == cudaSuccess ? XP_OK : static_cast<int>(err);
+}
+
 inline cudaStream_t as_stream(void *s) { return reinterpret_cast<cudaStream_t>(s); }
 
 inline bool aligned(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }

@@ -1505,18 +1505,18 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
   }
 }
 
-int set_smem(const void *fn, int bytes) {
-  if (bytes <= 48 * 1024) return XP_OK;
-  cudaError_t err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  return err == cudaSuccess ? XP_OK : static_cast<int>(err);
-}
+// CTAs of a kind that a device holds at once, for each device (0: not looked up yet).
+struct Fit {
+  static constexpr int kDevices = 64;
+  std::atomic<int> most[kDevices];
+};
 
 // `clusters` clusters of 2^log2c CTAs; where `fit` is not NULL no more than the device
-// holds at once (looked up once for a kernel and cluster size).  `early`: the launch
+// holds at once (looked up once for a kernel, cluster size and device).  `early`: the launch
 // may begin before the kernel before it has ended (it waits for that end itself).
-int launch(const void *fn, int64_t clusters, int log2c, int threads, int smem,
-           std::atomic<int> *fit, bool early, LowRankArgs &a, cudaStream_t s) {
-  int rc = set_smem(fn, smem);
+int launch(const void *fn, int64_t clusters, int log2c, int threads, int smem, int most_smem,
+           Fit *fit, bool early, LowRankArgs &a, cudaStream_t s) {
+  int rc = allow_smem(fn, smem, most_smem);
   if (rc) return rc;
   a.cluster_log2 = log2c;
   cudaLaunchConfig_t cfg = {};
@@ -1533,12 +1533,16 @@ int launch(const void *fn, int64_t clusters, int log2c, int threads, int smem,
   cfg.attrs = attr;
   cfg.numAttrs = early ? 2 : 1;
   if (fit) {
-    int most = fit->load(std::memory_order_relaxed);
+    int device = 0, most = 0;
+    cudaError_t err = cudaGetDevice(&device);
+    if (err != cudaSuccess) return static_cast<int>(err);
+    const bool kept = device < Fit::kDevices;
+    if (kept) most = fit->most[device].load(std::memory_order_relaxed);
     if (most == 0) {
-      cudaError_t err = cudaOccupancyMaxActiveClusters(&most, fn, &cfg);
+      err = cudaOccupancyMaxActiveClusters(&most, fn, &cfg);
       if (err != cudaSuccess) return static_cast<int>(err);
       if (most < 1) return XP_ERANGE;
-      fit->store(most, std::memory_order_relaxed);
+      if (kept) fit->most[device].store(most, std::memory_order_relaxed);
     }
     if (clusters > most) clusters = most;
   }
@@ -1563,18 +1567,18 @@ template <typename T, int kRB>
 int run_sized(LowRankArgs &a, cudaStream_t s) {
   const bool vec = a.vec_x && a.vec_a && a.vec_b && a.vec_y;
   if (a.M <= kRowsLimit) {
-    static std::atomic<int> fit[2][2];
+    static Fit fit[2][2];
     // Measured with 64 adapters (us, clusters of 8 / 4 / 2, ranks 16 and 64): 1 row 5.4 / 6.1 /
     // 8.3 and 6.3 / 7.6 / 11.2; 32 rows 6.6 / 6.5 / 8.6 and 8.3 / 7.9 / 11.4; 64 rows
     // 11.3 / 8.0 / 8.7 and 14.6 / 10.2 / 11.6; 256 rows 12.5 / 9.2 / 9.8 and 15.9 / 11.4 / 13.1.
     const int log2c = a.M <= 16 ? 3 : 2;
     const void *fn = vec ? (const void *)rows_kernel<T, kRB, true>
                          : (const void *)rows_kernel<T, kRB, false>;
-    return launch(fn, a.M, log2c, kThreads, RowsSmem<kRB>::kBytes, &fit[vec][log2c & 1], false, a,
-                  s);
+    constexpr int kBytes = RowsSmem<kRB>::kBytes;
+    return launch(fn, a.M, log2c, kThreads, kBytes, kBytes, &fit[vec][log2c & 1], false, a, s);
   }
   const int bytes = 12 * (a.slots + 1);
-  int rc = set_smem((const void *)plan_kernel, bytes);
+  int rc = allow_smem((const void *)plan_kernel, bytes, 12 * (XP_MAX_ADAPTER_SLOTS + 1));
   if (rc) return rc;
   plan_kernel<<<kPlanCtas, kPlanThreads, bytes, s>>>(a);
   rc = launch_status();
@@ -1606,8 +1610,9 @@ int run_sized(LowRankArgs &a, cudaStream_t s) {
   int smem = deep ? TileSmem<kRB, true, true>::kBytes
                   : (vec ? TileSmem<kRB, true, kRB == 8>::kBytes
                          : TileSmem<kRB, false, false>::kBytes);
-  if (shares && log2c > 0 && smem < kWholeSm) smem = kWholeSm;
-  return launch(fn, tiles, log2c, tile_threads(vec), smem, nullptr, true, a, s);
+  const int most = smem < kWholeSm ? kWholeSm : smem;
+  if (shares && log2c > 0) smem = most;
+  return launch(fn, tiles, log2c, tile_threads(vec), smem, most, nullptr, true, a, s);
 }
 
 template <typename T>

@@ -53,6 +53,7 @@ constexpr int kBackThreads = 256;  // the backward kernel's
 constexpr int backward_blocks(int vpl) {
   return vpl <= 8 ? 4 : (vpl <= 16 ? 3 : (vpl <= 32 ? 2 : 1));
 }
+constexpr int most_experts(int vpl) { return 32 * vpl; }
 constexpr int values_per_lane(int64_t E) {
   return E <= 64 ? 2 : (E <= 256 ? 8 : (E <= 512 ? 16 : (E <= 1024 ? 32 : 128)));
 }
@@ -759,13 +760,6 @@ __global__ void __launch_bounds__(kBackThreads, backward_blocks(VPL))
   }
 }
 
-int set_smem(const void *fn, size_t bytes) {
-  if (bytes <= 48 * 1024) return XP_OK;
-  cudaError_t err =
-      cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-  return err == cudaSuccess ? XP_OK : static_cast<int>(err);
-}
-
 // CTAs of the forward kernel.
 int64_t forward_ctas(int64_t T, int64_t E) {
   const int vpl = values_per_lane(E);
@@ -779,11 +773,15 @@ int launch_forward(const ForwardArgs &a, cudaStream_t s) {
   auto fn = a.given ? forward_kernel<T, VPL, VEC, true> : forward_kernel<T, VPL, VEC, false>;
   const int threads = forward_threads(VPL);
   const int64_t ctas = forward_ctas(a.T, a.E);
-  size_t smem = sizeof(int) * a.E;
-  if (a.loss)
-    smem += VPL > 32 ? (sizeof(double) + sizeof(float) * (threads / 32)) * a.E
-                     : sizeof(double) * (threads / 32) * Row<T, VPL, VEC>::kPlaces;
-  int rc = set_smem((const void *)fn, smem);
+  auto need = [&](int64_t E, bool loss) {
+    int64_t bytes = sizeof(int) * E;
+    if (loss)
+      bytes += VPL > 32 ? (sizeof(double) + sizeof(float) * (threads / 32)) * E
+                        : sizeof(double) * (threads / 32) * Row<T, VPL, VEC>::kPlaces;
+    return bytes;
+  };
+  const int64_t smem = need(a.E, a.loss != nullptr);
+  int rc = allow_smem((const void *)fn, smem, need(most_experts(VPL), true));
   if (rc) return rc;
   fn<<<static_cast<unsigned>(ctas), threads, smem, s>>>(a);
   rc = launch_status();
@@ -806,12 +804,13 @@ template <typename T, int VPL, bool VEC>
 int launch_backward(const BackwardArgs &a, cudaStream_t s) {
   auto fn = backward_kernel<T, VPL, VEC>;
   const int threads = kBackThreads;
-  const size_t smem = sizeof(float) * 32 * VPL * (1 + (a.grad_weights ? threads / 32 : 0));
-  int rc = set_smem((const void *)fn, smem);
+  const int64_t row = sizeof(float) * 32 * VPL, most = row * (1 + threads / 32);
+  const int64_t smem = a.grad_weights ? most : row;
+  int rc = allow_smem((const void *)fn, smem, most);
   if (rc) return rc;
   const int64_t want = (a.T + threads / 32 - 1) / (threads / 32);
-  const int64_t most = 148 * backward_blocks(VPL);
-  fn<<<static_cast<unsigned>(want < most ? want : most), threads, smem, s>>>(a);
+  const int64_t ctas = 148 * backward_blocks(VPL);
+  fn<<<static_cast<unsigned>(want < ctas ? want : ctas), threads, smem, s>>>(a);
   return launch_status();
 }
 
