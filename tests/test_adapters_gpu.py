@@ -715,3 +715,33 @@ def test_calls_of_several_threads():
         t.join()
     torch.cuda.synchronize()
     assert statuses == {4200: {native.XP_OK}, 8192: {native.XP_OK}}
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M, H, N, r", [(1100, 512, 256, 16), (1100, 1024, 256, 64),
+                                        (5000, 1021, 131, 13), (1100, 61, 95, 100),
+                                        (4000, 2048, 512, 128)])
+def test_waits_that_give_up_are_counted(dtype, M, H, N, r):
+    """With no time to wait, blocks give up: their columns are NaN, the others right, the host
+    can read how many did, and the next call finds everything as before."""
+    from vllm_expert_pager import adapters, native
+
+    S = 4
+    o, g = make(M, H, N, r, S, dtype, seed=M)
+    slots = torch.randint(-1, S, (M,), generator=g, device=DEV)
+    ids = slots.to(torch.int32)
+    want, bound = reference(o["y"], o["x"], o["a"], o["b"], slots, o["scale"])
+    clean = check(o, ids, slots, out=fresh(o))
+    before = adapters.wait_errors()
+    limit = native.lib().xp_low_rank_wait_limit(0)
+    try:
+        got = adapters.add_low_rank(o["y"], o["x"], o["a"], o["b"], ids, scale=o["scale"],
+                                    out=torch.zeros_like(o["y"]))
+        gave_up = adapters.wait_errors() - before
+    finally:
+        assert native.lib().xp_low_rank_wait_limit(limit) == 0
+    assert gave_up > 0 and got.isnan().any()
+    assert (got.isnan() | ((got.double() - want).abs() <= bound)).all()
+    assert torch.equal(got[slots < 0], o["y"][slots < 0])
+    assert torch.equal(check(o, ids, slots, out=fresh(o)), clean)
+    assert adapters.wait_errors() - before == gave_up

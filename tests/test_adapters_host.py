@@ -174,3 +174,14 @@ def test_one_row_may_be_updated_in_place_at_any_stride():
                                      "out": wide.as_strided((1, 24), (stride, 1))})
     with pytest.raises(ValueError, match="overlap"):
         adapters.add_low_rank(**{**o, "y": wide[:1, :24], "out": wide[:1, 1:25]})
+
+
+def test_wait_limit():
+    limit = native.lib().xp_low_rank_wait_limit
+    assert limit(-1) == 2 * 10**9
+    try:
+        assert limit(5) == 2 * 10**9 and limit(-7) == 5
+        assert limit(1 << 40) == 5 and limit(-1) == 2 * 10**9
+    finally:
+        limit(2 * 10**9)
+    assert native.lib().xp_low_rank_errors(None, None) == native.XP_EINVAL

@@ -70,6 +70,7 @@ struct LowRankArgs {
   int vec_x, vec_a, vec_b, vec_y;  // 16-byte accesses to x, A, B, and y with out
   int in_place;
   int cluster_log2;  // CTAs of a cluster
+  uint32_t wait_ns;  // after which a wait of tile_kernel gives up
   // The plan of tile_kernel.
   int32_t *perm;   // [M] rows by slot
   int4 *tiles;     // (slot, first place in perm, rows, -)
@@ -731,10 +732,14 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// mbarriers.  A wait gives up after kWaitNs or when another one of the block has:
-// it then sets *failed.
-constexpr uint64_t kWaitNs = 2000000000ull;
-constexpr int kFreePolls = 256;  // tries before the time is looked at
+// mbarriers.  A wait gives up after its limit or when another one of the block has: it then
+// sets *failed.  A block with such a wait adds 1 to wait_errors.
+constexpr uint32_t kWaitNs = 2000000000u;
+constexpr int kFreePolls = 16;        // tries before the time is looked at
+constexpr uint32_t kTryNs = 1000000;  // a try may be suspended for
+
+__device__ uint32_t wait_errors;
+std::atomic<uint32_t> wait_limit{kWaitNs};
 
 __device__ __forceinline__ void bar_init(uint32_t bar, int count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
@@ -754,29 +759,31 @@ __device__ __forceinline__ void bar_arrive_peer(uint32_t bar, int cta) {
 }
 
 template <bool kCluster = false>
-__device__ __forceinline__ bool bar_wait(uint32_t bar, int parity, volatile int *failed) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, int parity, uint32_t limit,
+                                         volatile int *failed) {
   uint64_t since = 0;
-  for (int i = 0;; ++i) {
+  const uint32_t hint = min(limit, kTryNs);
+  for (int i = limit ? 0 : kFreePolls;; ++i) {  // without a limit in time: a single try
     uint32_t done;
     if constexpr (kCluster)
       asm volatile(
           "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], "
-          "%2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+          "%2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
           : "=r"(done)
-          : "r"(bar), "r"(parity)
+          : "r"(bar), "r"(parity), "r"(hint)
           : "memory");
     else
       asm volatile(
-          "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+          "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
           "selp.u32 %0, 1, 0, p;\n\t}"
           : "=r"(done)
-          : "r"(bar), "r"(parity)
+          : "r"(bar), "r"(parity), "r"(hint)
           : "memory");
     if (done) return true;
     if (i < kFreePolls) continue;
     const uint64_t now = global_ns();
     if (i == kFreePolls) since = now;
-    if (*failed || now - since > kWaitNs) break;
+    if (*failed || now - since >= limit) break;
   }
   *failed = 1;
   return false;
@@ -908,7 +915,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
   const bool vec_y = kVec || a.vec_y;
   extern __shared__ unsigned char raw[];
   __shared__ int64_t rows[kTile];
-  __shared__ __align__(8) uint64_t bars[3 * kStages + 7 + 2 * S::kWords];
+  __shared__ __align__(8) uint64_t bars[3 * kStages + 8 + 2 * S::kWords];
   // Not kVec: where a row's first value lies in its words (bytes), and in the upper
   // half the bits to shift by; the rows' first values of out in this CTA's part.
   __shared__ uint32_t at_x[kVec ? 1 : kTile], at_y[kVec ? 1 : kTile], at_a[kVec ? 1 : S::kR],
@@ -932,11 +939,11 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
   const uint32_t ring = smem_addr(smem);
   // Stage filled; stage free after the first / the second product; v in tensor
   // memory; v's parts there; a block of out there, and read from it; the cluster's
-  // shares of v written; words arrived, and shifted.
+  // shares of v written; all matrix instructions over; words arrived, and shifted.
   const uint32_t full = smem_addr(bars), free1 = full + 8 * kStages, free2 = free1 + 8 * kStages;
   const uint32_t v_done = free2 + 8 * kStages, v_ready = v_done + 8, out_done = v_ready + 8,
-                 out_read = out_done + 16, shares = out_read + 16, words_full = shares + 8,
-                 words_free = words_full + 8 * S::kWords;
+                 out_read = out_done + 16, shares = out_read + 16, drained = shares + 8,
+                 words_full = drained + 8, words_free = words_full + 8 * S::kWords;
   volatile int *fail = &failed;
 
   if (tid < kTile) rows[tid] = a.perm[job.y + min(tid, n_rows - 1)];
@@ -959,6 +966,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
       bar_init(out_read + 8 * i, kOutWarps * 32);
     }
     bar_init(shares, C);
+    bar_init(drained, 1);
     for (int i = 0; i < S::kWords; ++i) {
       bar_init(words_full + 8 * i, kLoaders);
       bar_init(words_free + 8 * i, kLoaders);
@@ -1022,8 +1030,8 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
       if (use > 0) {
         const int before = (first + kStages - 1 - stage) / kStages;  // uses by the first product
         const bool ok = c - kStages < first
-                            ? bar_wait(free1 + 8 * stage, (use - 1) & 1, fail)
-                            : bar_wait(free2 + 8 * stage, (use - 1 - before) & 1, fail);
+                            ? bar_wait(free1 + 8 * stage, (use - 1) & 1, a.wait_ns, fail)
+                            : bar_wait(free2 + 8 * stage, (use - 1 - before) & 1, a.wait_ns, fail);
         if (!ok) return 0u;
       }
       return ring + stage * S::kStage;
@@ -1103,7 +1111,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
       const uint32_t words = ring + kStages * S::kStage + S::kShare;
       auto begin_words = [&](int c) {
         const int stage = c % S::kWords, use = c / S::kWords;
-        if (use > 0 && !bar_wait(words_free + 8 * stage, (use - 1) & 1, fail)) return 0u;
+        if (use > 0 && !bar_wait(words_free + 8 * stage, (use - 1) & 1, a.wait_ns, fail)) return 0u;
         return words + stage * S::kWordsStage;
       };
       // `bytes`: of the row's values from the block on.
@@ -1206,7 +1214,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
       };
       for (int c = 0; c < chunks; ++c) {
         const int stage = c % S::kWords;
-        if (!bar_wait(words_full + 8 * stage, (c / S::kWords) & 1, fail)) break;
+        if (!bar_wait(words_full + 8 * stage, (c / S::kWords) & 1, a.wait_ns, fail)) break;
         const uint32_t at = begin(c);
         if (!at) break;
         const unsigned char *from = words + stage * S::kWordsStage;
@@ -1258,7 +1266,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
       bool ok = true;
       for (int c = 0; c < first && ok; ++c) {
         const int stage = c % kStages;
-        ok = bar_wait(full + 8 * stage, (c / kStages) & 1, fail);
+        ok = bar_wait(full + 8 * stage, (c / kStages) & 1, a.wait_ns, fail);
         if (!ok) break;
         fence_async_proxy();
         tc_fence_after();
@@ -1270,11 +1278,11 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
       }
       if (ok && first > 0) tc_commit(v_done);
       if (ok && first == 0) bar_arrive(v_done);
-      ok = ok && bar_wait(v_ready, 0, fail);
+      ok = ok && bar_wait(v_ready, 0, a.wait_ns, fail);
       for (int c = first; c < chunks && ok; ++c) {
         const int stage = c % kStages, i = c - first, half = i & 1;
-        ok = bar_wait(full + 8 * stage, (c / kStages) & 1, fail) &&
-             (i < 2 || bar_wait(out_read + 8 * half, (i / 2 - 1) & 1, fail));
+        ok = bar_wait(full + 8 * stage, (c / kStages) & 1, a.wait_ns, fail) &&
+             (i < 2 || bar_wait(out_read + 8 * half, (i / 2 - 1) & 1, a.wait_ns, fail));
         if (!ok) break;
         fence_async_proxy();
         tc_fence_after();
@@ -1293,6 +1301,11 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
           }
         tc_commit(out_done + 8 * half);
       }
+      // What has been issued reads and writes memory that is given back below, though the
+      // warps that wait for its results may have given up.
+      volatile int never = 0;
+      tc_commit(drained);
+      bar_wait(drained, 0, kWaitNs, &never);
     }
     __syncwarp();
   } else {
@@ -1301,7 +1314,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
     const int row = tid & 127, side = warp >> 2;
     const uint32_t my_tmem = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const float scale = a.scale ? a.scale[s] : 1.0f;
-    bool ok = __all_sync(kFull, bar_wait(v_done, 0, fail));
+    bool ok = __all_sync(kFull, bar_wait(v_done, 0, a.wait_ns, fail));
     tc_fence_after();
     constexpr int kMine = (kRB + 1) / 2;  // blocks of 16 ranks: every other one is this side's
     float u[kMine][16];
@@ -1330,7 +1343,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
         asm volatile("fence.acq_rel.cluster;" ::: "memory");
         bar_arrive_peer(shares, tid);
       }
-      ok = __all_sync(kFull, ok && bar_wait<true>(shares, 0, fail));
+      ok = __all_sync(kFull, ok && bar_wait<true>(shares, 0, a.wait_ns, fail));
       if (ok) {
 #pragma unroll
         for (int i = 0; i < kMine; ++i)
@@ -1396,8 +1409,8 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
     // After a wait gave up, warps that meet others at a barrier still do.
     for (int c = first; c < chunks && (ok || !vec_y); ++c) {
       const int stage = c % kStages, i = c - first, half = i & 1;
-      ok = __all_sync(kFull, ok && bar_wait(out_done + 8 * half, (i / 2) & 1, fail) &&
-                                 bar_wait(full + 8 * stage, (c / kStages) & 1, fail));
+      ok = __all_sync(kFull, ok && bar_wait(out_done + 8 * half, (i / 2) & 1, a.wait_ns, fail) &&
+                                 bar_wait(full + 8 * stage, (c / kStages) & 1, a.wait_ns, fail));
       if (!ok && vec_y) break;
       tc_fence_after();
       unsigned char *ys = smem + stage * S::kStage + S::kY;
@@ -1487,6 +1500,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
       if (ok && lane == 0) bar_arrive(free2 + 8 * stage);
     }
   }
+  __syncwarp();  // lanes may have given up apart
   tc_fence_before();
   if (shared_v)
     cluster.sync();  // a CTA's barriers and its share stay until the cluster has used them
@@ -1498,6 +1512,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
                  "n"(tmem_cols(kRB)));
   }
   if (failed) {  // a wait gave up: the rows must not pass for results
+    if (tid == 0) atomicAdd(&wait_errors, 1u);
     for (int i = 0; i < n_rows; ++i)
       for (int64_t n = static_cast<int64_t>(n0) * kNBlock + tid;
            n < min(a.N, static_cast<int64_t>(n1) * kNBlock); n += blockDim.x)
@@ -1659,6 +1674,7 @@ extern "C" int xp_add_low_rank(const void *x, int64_t x_stride, const void *y, i
   p.vec_a = aligned(a, 16) && H % 8 == 0;
   p.vec_b = aligned(b, 16) && r % 8 == 0;
   p.vec_y = aligned(y, 16) && aligned(out, 16) && y_stride % 8 == 0 && out_stride % 8 == 0;
+  p.wait_ns = wait_limit.load(std::memory_order_relaxed);
   p.in_place = y == out && (y_stride == out_stride || M == 1);
   if (M > kRowsLimit) {
     unsigned char *at = static_cast<unsigned char *>(scratch);
@@ -1668,4 +1684,17 @@ extern "C" int xp_add_low_rank(const void *x, int64_t x_stride, const void *y, i
   }
   return dtype == XP_BF16 ? run_typed<__nv_bfloat16>(p, as_stream(stream))
                           : run_typed<__half>(p, as_stream(stream));
+}
+
+extern "C" int xp_low_rank_errors(uint32_t *count, void *stream) {
+  if (!count) return XP_EINVAL;
+  cudaError_t err = cudaMemcpyFromSymbolAsync(count, wait_errors, sizeof(*count), 0,
+                                              cudaMemcpyDeviceToHost, as_stream(stream));
+  if (err == cudaSuccess) err = cudaStreamSynchronize(as_stream(stream));
+  return err == cudaSuccess ? XP_OK : static_cast<int>(err);
+}
+
+extern "C" int64_t xp_low_rank_wait_limit(int64_t ns) {
+  if (ns < 0) return wait_limit.load(std::memory_order_relaxed);
+  return wait_limit.exchange(static_cast<uint32_t>(ns < kWaitNs ? ns : kWaitNs));
 }

@@ -13,6 +13,8 @@ the row copy (``gather.py``) that page experts.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from vllm_expert_pager import native
@@ -42,8 +44,25 @@ def add_low_rank(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     that would need a gradient, or with a dual tensor of forward-mode
     derivatives, is refused, and a backward pass that saved the
     values which ``out`` had before raises, as after torch's own updates in place.
+    Rows may hold NaN that the operands do not explain only if ``wait_errors`` has
+    risen.
     """
     return native.torch_ops().add_low_rank(y, x, a, b, ids, scale, slot_map, out)
+
+
+def wait_errors(device: torch.device | None = None) -> int:
+    """Blocks of ``add_low_rank`` that gave up waiting on ``device`` (the current one) so far.
+
+    The parts of a block of a call with more than 1024 rows wait for one another, 2
+    seconds at most; a block that gives up fills its part of ``out`` with NaN.  Waits
+    for the current stream, so it is not for a capture.
+    """
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+    count = ctypes.c_uint32()
+    with torch.cuda.device(device):
+        native.check(native.lib().xp_low_rank_errors(ctypes.byref(count),
+                                                     native.stream_of(device)), "wait_errors")
+    return count.value
 
 
 class AdapterPager:

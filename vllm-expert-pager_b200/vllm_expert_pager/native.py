@@ -78,6 +78,8 @@ _SIGNATURES = {
     "xp_low_rank_scratch_bytes": (_i64, [_i64, _i64]),
     "xp_add_low_rank": (_i32, [_p, _i64, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _i64, _p, _p,
                                _i64, _p, _p, _i32, _p, _i32, _i64, _p, _i64, _p]),
+    "xp_low_rank_errors": (_i32, [ctypes.POINTER(ctypes.c_uint32), _p]),
+    "xp_low_rank_wait_limit": (_i64, [_i64]),
     "xp_pinned_alloc": (_i32, [_i64, _i32, ctypes.POINTER(_p), ctypes.POINTER(_p)]),
     "xp_pinned_free": (_i32, [_p, _i64]),
     "xp_device_pointer": (_i32, [_p, ctypes.POINTER(_p)]),
