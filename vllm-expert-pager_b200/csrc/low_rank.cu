@@ -993,7 +993,8 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
 
   const T *A = static_cast<const T *>(a.a) + static_cast<int64_t>(s) * a.r * a.H;
   const T *B = static_cast<const T *>(a.b) + static_cast<int64_t>(s) * a.r * a.N;
-  // This CTA's blocks of 64 along H and along N.
+  // This CTA's blocks of 64 along H (where it is split there are more than CTAs) and along N
+  // (there may be none).
   const uint32_t nb_all = static_cast<uint32_t>((a.N + kNBlock - 1) / kNBlock);
   const int k0 = shared_v ? kb_all * rank >> log2c : 0;
   const int k1 = shared_v ? kb_all * (rank + 1) >> log2c : kb_all;
@@ -1276,8 +1277,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
           tc_mma(tmem, operand(at + 32 * i), operand(at + S::kA + 32 * i), kWhat1, c > 0 || i > 0);
         tc_commit(free1 + 8 * stage);
       }
-      if (ok && first > 0) tc_commit(v_done);
-      if (ok && first == 0) bar_arrive(v_done);
+      if (ok) tc_commit(v_done);
       ok = ok && bar_wait(v_ready, 0, a.wait_ns, fail);
       for (int c = first; c < chunks && ok; ++c) {
         const int stage = c % kStages, i = c - first, half = i & 1;
@@ -1322,7 +1322,7 @@ __global__ void __launch_bounds__(tile_threads(kVec), kVec && kRB <= 4 && !kDeep
     for (int i = 0; i < kMine; ++i) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) u[i][j] = 0.0f;
-      if (ok && first > 0 && 2 * i + side < kRB) tc_load16(u[i], my_tmem + (2 * i + side) * 16);
+      if (ok && 2 * i + side < kRB) tc_load16(u[i], my_tmem + (2 * i + side) * 16);
     }
     if (shared_v) {
       // The cluster's shares of v, added in the order of its CTAs.  Four ranks of all
