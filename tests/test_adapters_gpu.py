@@ -745,3 +745,34 @@ def test_waits_that_give_up_are_counted(dtype, M, H, N, r):
     assert torch.equal(got[slots < 0], o["y"][slots < 0])
     assert torch.equal(check(o, ids, slots, out=fresh(o)), clean)
     assert adapters.wait_errors() - before == gave_up
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M, H, N, r, S", [
+    # Clusters of four: aligned and not, columns for some CTAs only, H just split and not.
+    (1100, 2048, 192, 8, 8), (1100, 2048, 100, 128, 4), (1100, 1021, 2047, 13, 8),
+    (1025, 769, 64, 32, 2), (1300, 768, 136, 64, 8), (1300, 832, 136, 64, 8),
+    # Of two.
+    (5000, 1024, 192, 64, 8), (5000, 1021, 131, 16, 8), (5000, 832, 64, 128, 8),
+    # One CTA a tile, one and two of them on an SM, ranks of every kind.
+    (16384, 1024, 128, 64, 8), (16384, 1024, 72, 16, 8), (16384, 832, 128, 128, 8),
+    (16384, 1021, 131, 40, 8), (24000, 1024, 128, 64, 8), (24000, 896, 64, 32, 8),
+    # More slots than tiles.
+    (1600, 1024, 72, 16, 600)])
+def test_long_batches_of_wide_rows(dtype, M, H, N, r, S):
+    """Rows so wide that the CTAs of a tile share their sums."""
+    from vllm_expert_pager import adapters
+
+    o, g = make(M, H, N, r, S, dtype, seed=M + r)
+    i = torch.arange(M, device=DEV)
+    for slots in (torch.randint(-1, S, (M,), generator=g, device=DEV), i * 5 // M % S,
+                  torch.full((M,), S - 1, device=DEV)):
+        ids = slots.to(torch.int32)
+        first = check(o, ids, slots, out=fresh(o))
+        for _ in range(3):
+            again = adapters.add_low_rank(o["y"], o["x"], o["a"], o["b"], ids, scale=o["scale"],
+                                          out=fresh(o))
+            assert torch.equal(again, first)
+        y = o["y"].clone()
+        adapters.add_low_rank(y, o["x"], o["a"], o["b"], ids, scale=o["scale"])
+        assert torch.equal(y, first)
