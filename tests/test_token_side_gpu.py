@@ -187,3 +187,26 @@ def test_router_tuning_over_paged_experts(layer):
     got = float((gate.grad.double() * way).sum())
     # Differences: h^2; the logits' 32-bit products of 2048 terms: 2048 steps of 2^-23.
     assert abs(got - slope) <= 4e-4 * float((gate.grad * way).abs().sum())
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs a second GPU")
+def test_tensors_of_another_device_than_the_current_one():
+    from vllm_expert_pager import adapters, routing
+
+    def run(dev):
+        g = torch.Generator().manual_seed(3)
+        logits = torch.randn((3000, 256), generator=g).to(dev).requires_grad_()
+        r = routing.route(logits, 8, balance=True)
+        grad, = torch.autograd.grad(r.loss + r.weights[:, 0].sum(), logits)
+        outs = [r.weights.detach(), r.ids, r.counts, r.loss.detach(), grad]
+        for M in (5, 1500):
+            y, x, a, b = (torch.randn(s, generator=g).to(dev, torch.bfloat16) for s in
+                          ((M, 96), (M, 1024), (4, 16, 1024), (4, 96, 16)))
+            ids = (torch.arange(M) % 5 - 1).to(dev)
+            outs.append(adapters.add_low_rank(y, x, a, b, ids))
+        assert adapters.wait_errors(dev) == 0
+        return [t.cpu() for t in outs]
+
+    with torch.cuda.device(0):
+        here, there = run(torch.device("cuda", 0)), run(torch.device("cuda", 1))
+    assert all(torch.equal(u, v) for u, v in zip(here, there))

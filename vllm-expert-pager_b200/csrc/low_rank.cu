@@ -16,7 +16,7 @@
 //    instruction's 16-row operand and the rows as its 8 columns (mma.sync: at 8
 //    columns the tensor cores wait for memory in any form).  Which rows belong
 //    together each cluster finds out by itself from the ids, so the call is one
-//    launch.  B200, 256 rows of 100 adapters, rank 64, 2048 -> 1024: 15.4 us, of
+//    launch.  B200, 256 rows of 100 adapters, rank 64, 2048 -> 1024: 15.8 us, of
 //    which A comes at HBM's rate for 5.
 //  * tile_kernel: long batches.  Bound by reading x and y and writing out.  A
 //    small launch sorts the rows by slot; then a CTA (or a cluster, where there
@@ -24,7 +24,7 @@
 //    B and y, through one ring of shared-memory stages, one thread issues tcgen05
 //    instructions with the sums in tensor memory, and eight warps make v's parts
 //    and write out.  The second product's operands are on their way while the
-//    first one ends.  B200, 16384 rows, rank 64, 2048 -> 2048: 53 us against 32 of
+//    first one ends.  B200, 16384 rows, rank 64, 2048 -> 2048: 52 us against 32 of
 //    HBM; a tile's chain of 64 blocks alone takes 45.  (mma.sync on 64-row tiles took
 //    87: its instructions alone fill the tensor pipe for 29 us at that rank.)
 #include <cooperative_groups.h>
@@ -45,8 +45,10 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 // rows_kernel up to here.  Measured at 2048 -> 2048, rank 16 (us, rows_kernel /
-// tile_kernel): 512 rows of 4 adapters 9.4 / 18.0, of 256 adapters 25.5 / 138; 1024 rows
-// 16.7 / 18.1 and 29 / 139; 1536 rows 22.7 / 18.6 and 34 / 139.
+// tile_kernel): 512 rows of 4 adapters 9.5 / 18.7, of 256 adapters 26 / 72; 1024 rows
+// 17.2 / 19.0 and 30 / 72; 1536 rows 23.2 / 19.3 and 35 / 72.  2048 -> 1024, rank 64: 1024
+// rows 21 / 21 and 45 / 67; 1536 rows 32 / 21 and 50 / 67.  The bound knows the rows alone:
+// right for few adapters, it gives 1536 rows of 256 adapters to the slower kernel.
 constexpr int kRowsLimit = 1024;
 constexpr int kGroup = 8;         // rows of a cluster of rows_kernel
 constexpr int kRowStages = 3;     // its ring
@@ -868,9 +870,11 @@ constexpr int kLoadWarps = 4;
 constexpr int kLoaders = kLoadWarps * 32;
 constexpr int kShiftWarps = 4;               // where rows lie at any place
 constexpr int kNBlock = 64;                  // columns of out in a stage
-// Blocks of 64 of H that are not split.  Measured with 2048 rows, rank 16, 2048 columns (us,
-// whole / split): H 256 16.5 / 21.8, 512 17.8 / 21.3, 768 19.3 / 21.7, 1024 21.2 / 21.8,
-// 2048 27.2 / 22.7; with 4096 rows 768 21.6 / 21.2.
+// Blocks of 64 of H that are not split.  Measured with 2048 columns, 6 adapters in 8 slots
+// (us, whole / split): rank 16, 1100 rows, H 512 14.1 / 17.0, 768 15.3 / 17.4; 2048 rows, 256
+// 15.6 / 17.0, 512 17.5 / 17.2, 768 19.0 / 17.4, 1024 20.6 / 18.0; 4096 rows, 256 22.9 / 23.7,
+// 512 26.2 / 24.5, 768 29.4 / 25.2, 1024 33.1 / 25.9; rank 64, H 512, 1100 rows 15.9 / 21.3,
+// 2048 20.3 / 21.8, 4096 29.7 / 27.5.  Few rows bear a longer whole H than many.
 constexpr uint32_t kWholeBlocks = 12;
 // Tensor memory: v's sums, and when they have been read two blocks of out in their place;
 // behind them v's parts, two values a column.  All parts are there, none in shared memory:
@@ -1583,9 +1587,9 @@ int run_sized(LowRankArgs &a, cudaStream_t s) {
   const bool vec = a.vec_x && a.vec_a && a.vec_b && a.vec_y;
   if (a.M <= kRowsLimit) {
     static Fit fit[2][2];
-    // Measured with 64 adapters (us, clusters of 8 / 4 / 2, ranks 16 and 64): 1 row 5.4 / 6.1 /
-    // 8.3 and 6.3 / 7.6 / 11.2; 32 rows 6.6 / 6.5 / 8.6 and 8.3 / 7.9 / 11.4; 64 rows
-    // 11.3 / 8.0 / 8.7 and 14.6 / 10.2 / 11.6; 256 rows 12.5 / 9.2 / 9.8 and 15.9 / 11.4 / 13.1.
+    // Measured with 64 adapters (us, clusters of 8 / 4 / 2, ranks 16 and 64): 1 row 5.6 / 6.3 /
+    // 8.7 and 6.4 / 7.7 / 11.5; 32 rows 6.7 / 6.7 / 8.9 and 8.4 / 8.2 / 11.7; 64 rows
+    // 11.4 / 8.2 / 9.0 and 14.8 / 10.3 / 11.8; 256 rows 12.6 / 9.4 / 10.2 and 16.0 / 11.6 / 13.4.
     const int log2c = a.M <= 16 ? 3 : 2;
     const void *fn = vec ? (const void *)rows_kernel<T, kRB, true>
                          : (const void *)rows_kernel<T, kRB, false>;
@@ -1606,8 +1610,8 @@ int run_sized(LowRankArgs &a, cudaStream_t s) {
   const bool shares = a.H > 64 * static_cast<int64_t>(kWholeBlocks);
   // As large a cluster for a tile as leaves all tiles on the device at once, if half
   // of the slots are in use (the host does not know).  Measured at 2048 -> 2048, 6 adapters
-  // in 8 slots (us, clusters of 1 / 2 / 4): rank 16, 3000 rows 44 / 29 / 22, 4096 45 / 30 / 37
-  // (more tiles than fit), 8192 45 / 31 / 40, 12000 46 / 57 / 57; rank 64, 8192 49 / 34 / 48.
+  // in 8 slots (us, clusters of 1 / 2 / 4): rank 16, 3000 rows 44 / 28 / 20, 4096 44 / 29 / 35
+  // (more tiles than fit), 8192 45 / 31 / 43, 12000 46 / 63 / 62; rank 64, 8192 51 / 34 / 52.
   // At 512 -> 2048, nothing exchanged and two CTAs on an SM, 2048 rows take 18 in clusters of 8.
   const int64_t full = (a.M + kTile - 1) / kTile, guess = full + a.slots / 2;
   const bool two = vec && kRB <= 4;  // two CTAs fit on an SM
@@ -1617,7 +1621,7 @@ int run_sized(LowRankArgs &a, cudaStream_t s) {
   else
     for (log2c = 3; log2c > 0 && guess << log2c > (two ? 296 : 148);) --log2c;
   // One CTA on an SM with a deep ring up to as many tiles as SMs, then two (16384 rows, rank
-  // 64, 2048 -> 2048: 52 / 62 us; 24000 rows: 96 / 84).
+  // 64, 2048 -> 2048: 52 / 62 us; 24000 rows: 97 / 82).
   const bool deep = vec && (!two || (shares && guess << log2c <= 148));
   const void *fn = deep ? (const void *)tile_kernel<T, kRB, true, true>
                         : (vec ? (const void *)tile_kernel<T, kRB, true, kRB == 8>

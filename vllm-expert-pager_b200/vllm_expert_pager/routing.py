@@ -48,7 +48,8 @@ def route(logits: torch.Tensor, topk: int, *, renormalize: bool = True,
     chosen experts, divided by their sum with ``renormalize``.  A NaN logit is
     chosen first and makes its token's weights NaN.  ``valid`` (bool ``[T]``)
     marks the rows that hold a token: the others get ids -1 and weights 0, and
-    nothing of them is read or counted.
+    nothing of them is read or counted.  A probability ``exp(l - max) / sum`` is exact to
+    about ``10 + 2 (max - l)`` steps of 2^-23, and 0 below 2^-126.
 
     ``counts[e]`` is the number of tokens routed to expert ``e``.  ``balance``
     adds ``loss = E * sum_e f_e P_e``, ``f_e`` the share of choices that went to
