@@ -372,7 +372,7 @@ int xp_add_low_rank(const void *x, int64_t x_stride, const void *y, int64_t y_st
  * wait ends after 2 seconds at the latest, if the GPU is held up that long: the block then
  * writes NaN to its part of out and counts itself.  xp_low_rank_errors stores the blocks
  * that gave up on the current device so far, after what is on the stream (for which it
- * waits).  xp_low_rank_wait_limit sets the limit of all later launches in nanoseconds (2 *
+ * waits; a stream in capture is XP_EINVAL).  xp_low_rank_wait_limit sets the limit of all later launches in nanoseconds (2 *
  * 10^9 at most; 0: a wait that is not over at once gives up) and returns the one before; a
  * negative value only returns it. */
 int xp_low_rank_errors(uint32_t *count, void *stream);

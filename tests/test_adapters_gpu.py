@@ -776,3 +776,21 @@ def test_long_batches_of_wide_rows(dtype, M, H, N, r, S):
         y = o["y"].clone()
         adapters.add_low_rank(y, o["x"], o["a"], o["b"], ids, scale=o["scale"])
         assert torch.equal(y, first)
+
+
+def test_wait_errors_leave_a_capture_alone():
+    from vllm_expert_pager import adapters
+
+    o, _ = make(1100, 64, 32, 8, 2, torch.bfloat16)
+    ids = torch.zeros((1100,), dtype=torch.int32, device=DEV)
+    want = adapters.add_low_rank(o["y"], o["x"], o["a"], o["b"], ids, out=fresh(o))
+    out = fresh(o)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        adapters.add_low_rank(o["y"], o["x"], o["a"], o["b"], ids, out=out)
+        with pytest.raises(ValueError, match="wait_errors failed"):
+            adapters.wait_errors()
+    before = adapters.wait_errors()
+    graph.replay()
+    assert adapters.wait_errors(DEV) == before and torch.equal(out, want)

@@ -6,7 +6,8 @@
 // whole, as the sum of three 16-bit parts (8 or 11 bits each; two of bfloat16 would
 // lose 2^-16 of v, which shows where v's terms cancel).  float16 parts are taken of v
 // times the power of two that brings the row's largest magnitude to 2^14, so that
-// neither end of the type's range is left.
+// neither end of the type's range is left; its least value then is 2^-38 of that magnitude,
+// and bounds what values far below it keep.
 //
 // Two kernels, by the number of rows (see kRowsLimit):
 //
@@ -1692,7 +1693,12 @@ extern "C" int xp_add_low_rank(const void *x, int64_t x_stride, const void *y, i
 
 extern "C" int xp_low_rank_errors(uint32_t *count, void *stream) {
   if (!count) return XP_EINVAL;
-  cudaError_t err = cudaMemcpyFromSymbolAsync(count, wait_errors, sizeof(*count), 0,
+  // A wait for a stream would end its capture.
+  cudaStreamCaptureStatus capture;
+  cudaError_t err = cudaStreamIsCapturing(as_stream(stream), &capture);
+  if (err != cudaSuccess) return static_cast<int>(err);
+  if (capture != cudaStreamCaptureStatusNone) return XP_EINVAL;
+  err = cudaMemcpyFromSymbolAsync(count, wait_errors, sizeof(*count), 0,
                                               cudaMemcpyDeviceToHost, as_stream(stream));
   if (err == cudaSuccess) err = cudaStreamSynchronize(as_stream(stream));
   return err == cudaSuccess ? XP_OK : static_cast<int>(err);

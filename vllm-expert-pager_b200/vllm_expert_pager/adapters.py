@@ -55,7 +55,7 @@ def wait_errors(device: torch.device | None = None) -> int:
 
     The parts of a block of a call with more than 1024 rows wait for one another, 2
     seconds at most; a block that gives up fills its part of ``out`` with NaN.  Waits
-    for the current stream, so it is not for a capture.
+    for the current stream; during its capture it raises ValueError.
     """
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
     count = ctypes.c_uint32()
